@@ -49,8 +49,9 @@ void OMShutdownAccelMI355X(void);
 /* Version of this runtime, encoded 0x00MMmmpp.  The major number changes with
  * every change of an existing signature (1: the fused entry points gained
  * `activation`), the minor number with every entry point added that
- * generated code may call (1: om_mi355x_SetQuantMode, activation = 2). */
-#define OM_MI355X_VERSION 0x00010100ULL
+ * generated code may call (1: om_mi355x_SetQuantMode, activation = 2; 2: the
+ * ops of decoder layers held in 8 and 4 bits). */
+#define OM_MI355X_VERSION 0x00010200ULL
 
 /* ---- compiler options that change this path's arithmetic ------------------ */
 /* The reference compiles QuantizeLinear / DynamicQuantizeLinear differently
@@ -225,6 +226,96 @@ void om_mi355x_DynQuantMatMulDequantLimits(OMTensor *y, OMTensor *y_limits,
     const OMTensor *x, const OMTensor *x_limits, const OMTensor *b,
     const OMTensor *b_zp, const OMTensor *b_scale, const OMTensor *bias,
     int64_t activation);
+
+/* ---- decoder layers in 8 and 4 bits --------------------------------------- */
+/* Ops of the layers of large language models.  The reference has no lowering
+ * for them; they keep this file's conventions.  Activations x, q, k, v and
+ * results y are f32, f16 or bf16 ("float" below), sums, scales and softmax
+ * statistics are f32 whatever their type, and results are rounded once. */
+
+/* Float to 8-bit floating point (e4m3) with one scale for each block of 128:
+ *   scale = max(max |x| / 448, 2^-126) over the block,  y = e4m3(x / scale),
+ * each f32 operation rounded to nearest even, y saturated at 448.  NaN is left
+ * out of the maximum and stays NaN; a block that holds an infinity has an
+ * infinite scale and NaN in the infinity's place.
+ * x: float [.., K]; y: f8e4m3fn of x's shape.
+ * block_rows 1:   a block is 128 neighbouring elements of a row (the last one
+ *                 of a row what is left of it); y_scale f32 [.., ceil(K/128)];
+ *            128: x is [N, K] and a block 128 x 128, for weights; y_scale f32
+ *                 [ceil(N/128), ceil(K/128)]. */
+void om_mi355x_DynamicQuantizeBlocks(OMTensor *y, OMTensor *y_scale,
+    const OMTensor *x, int64_t block_rows);
+
+/* Product of two such operands, the right-hand one [N, K] as weights lie in
+ * memory (onnx.Gemm with transB = 1):
+ *   y[m,n] = act(sum_kb a_scale[m,kb] b_scale[n/128,kb]
+ *                  sum_{k in kb} a[m,k] b[n,k] + bias[n])
+ * y: float [.., N]; a: f8e4m3fn [.., K], its leading dimensions folded into M;
+ * a_scale: f32 [.., ceil(K/128)]; b: f8e4m3fn [N, K]; b_scale: f32
+ * [ceil(N/128), ceil(K/128)]; bias: NULL, f32 scalar or [N]; activation as for
+ * om_mi355x_MatMulIntegerDequant.
+ * Where y has 16 bits and more than 64 rows, the products of a block are added
+ * by matrix instructions for 8-bit operands, whose sums are off by up to 1e-4
+ * of the result's magnitude, less than y's own rounding; otherwise they are
+ * f32 sums. */
+void om_mi355x_MatMulBlocks(OMTensor *y, const OMTensor *a,
+    const OMTensor *a_scale, const OMTensor *b, const OMTensor *b_scale,
+    const OMTensor *bias, int64_t activation);
+
+/* onnx.RotaryEmbedding.  x: float [B, H, S, D], or [B, S, H * D] with num_heads
+ * = H; y like x (it may be x).  The first rotary_embedding_dim elements of a
+ * head (0: all) are rotated in pairs, (2 i, 2 i + 1) if interleaved, otherwise
+ * (i, i + rotary_embedding_dim / 2), the others pass through.
+ * cos_cache, sin_cache: f32 (whatever x's type) [positions,
+ * rotary_embedding_dim / 2] with position_ids i64 [B, S], or
+ * [B, S, rotary_embedding_dim / 2] with position_ids NULL.  A token whose
+ * position the tables do not hold gets NaN. */
+void om_mi355x_RotaryEmbedding(OMTensor *y, const OMTensor *x,
+    const OMTensor *cos_cache, const OMTensor *sin_cache,
+    const OMTensor *position_ids, int64_t interleaved, int64_t num_heads,
+    int64_t rotary_embedding_dim);
+
+/* The 4-bit cache of keys and values.  A row (one token in one head) of D
+ * elements, D = 64, 96, 128, 192 or 256, is held in groups of 32: codes 0 .. 15
+ * with a scale s and a lowest value m in f16, x ~ s * code + m.
+ *   codes  ui8 [pages, H, page_size, D / 2]: with G = D / 32, byte n * G + g of
+ *          a row holds elements 32 g + 2 n (low half) and 32 g + 2 n + 1;
+ *   scales f16 [pages, H, page_size, G, 2]: (s, m).
+ * page_table: i32 [B, n], token t of sequence b lies in slot t % page_size of
+ * page page_table[b, t / page_size] (page_size a multiple of 16), or NULL:
+ * sequence b has page b.  past: i32 [B], tokens in front of the new ones.
+ * counts: i32 [B], how many of the S rows of a sequence are new tokens, or
+ * NULL: all S.  New token i of sequence b is token past[b] + i.
+ * Tables, past and counts that lie in host memory are checked (EINVAL); in GPU
+ * memory a token without a place in the cache is not stored, and not seen.
+ *
+ * om_mi355x_CacheAppend4 stores rows i < counts[b] and leaves everything else
+ * as it was.  k, v: float [B, H, S, D] or [B, S, H * D].  Of each group, x
+ * limited to +-65504: m = f16(min x), s = f16(max((max x - m) * f32(1/15), 0)),
+ * code = rint((x - m) / s) limited to 0 .. 15 (0 where s is 0), in f32 operations; a
+ * group that holds a NaN has s = m = NaN and codes 0. */
+void om_mi355x_CacheAppend4(OMTensor *k_codes, OMTensor *k_scales,
+    OMTensor *v_codes, OMTensor *v_scales, const OMTensor *k,
+    const OMTensor *v, const OMTensor *page_table, const OMTensor *past,
+    const OMTensor *counts);
+
+/* Attention of new tokens over the cache, which holds them already:
+ *   y = softmax(q khat^T * scale) vhat, khat and vhat what the cache stands for.
+ * q, y: float [B, Hq, S, D] or [B, S, Hq * D]; query head j attends to head
+ * j / (Hq / H) of the cache.  scale: f32 scalar, or NULL: 1 / sqrt(D).
+ * The query of new token i (token t = past[b] + i) sees the keys of tokens
+ *   up to t if causal, otherwise all of them (past[b] + counts[b]);
+ *   from t - window + 1 on, if window > 0;
+ *   from starts[b] on (i32 [B] or NULL: sequences padded on the left).
+ * A query that sees none has y = 0; what lies in places that a query does not
+ * see, NaN or infinite, does not reach its result.  Rows i >= counts[b] of y
+ * stay as they were. */
+void om_mi355x_CacheAttention4(OMTensor *y, const OMTensor *q,
+    const OMTensor *k_codes, const OMTensor *k_scales,
+    const OMTensor *v_codes, const OMTensor *v_scales,
+    const OMTensor *page_table, const OMTensor *past, const OMTensor *counts,
+    const OMTensor *starts, const OMTensor *scale, int64_t causal,
+    int64_t window);
 
 /* ---- residency ---------------------------------------------------------- */
 /* Declares that the host buffer behind `t` never changes for the life of the

@@ -27,7 +27,10 @@ typedef enum {
   OM_MI355X_TYPE_UINT8 = 2,
   OM_MI355X_TYPE_INT8 = 3,
   OM_MI355X_TYPE_INT32 = 6,
-  OM_MI355X_TYPE_INT64 = 7
+  OM_MI355X_TYPE_INT64 = 7,
+  OM_MI355X_TYPE_FLOAT16 = 10,
+  OM_MI355X_TYPE_BFLOAT16 = 16,
+  OM_MI355X_TYPE_FLOAT8E4M3FN = 17
 } OM_MI355X_DATA_TYPE;
 
 /* include/onnx-mlir/Runtime/OMTensor.h:92,159,168,197,228,279,319,327,335 */

@@ -30,8 +30,12 @@ static int64_t dtype_size(int dtype) {
   case OM_MI355X_TYPE_FLOAT:
   case OM_MI355X_TYPE_INT32:
     return 4;
+  case OM_MI355X_TYPE_FLOAT16:
+  case OM_MI355X_TYPE_BFLOAT16:
+    return 2;
   case OM_MI355X_TYPE_UINT8:
   case OM_MI355X_TYPE_INT8:
+  case OM_MI355X_TYPE_FLOAT8E4M3FN:
     return 1;
   case OM_MI355X_TYPE_INT64:
     return 8;

@@ -31,6 +31,7 @@
 #include <unordered_set>
 #include <vector>
 
+#include "llm_kernels.h"
 #include "om_kernels.h"
 #include "om_mi355x.h"
 
@@ -768,8 +769,14 @@ size_t dtype_bytes(int dt) {
   case OM_MI355X_TYPE_FLOAT:
   case OM_MI355X_TYPE_INT32:
     return 4;
+  case OM_MI355X_TYPE_INT64:
+    return 8;
+  case OM_MI355X_TYPE_FLOAT16:
+  case OM_MI355X_TYPE_BFLOAT16:
+    return 2;
   case OM_MI355X_TYPE_UINT8:
   case OM_MI355X_TYPE_INT8:
+  case OM_MI355X_TYPE_FLOAT8E4M3FN:
     return 1;
   default:
     return 0;
@@ -1104,6 +1111,17 @@ struct Call {
     backs.push_back(Back{v.data, d, v.bytes});
     back_bytes += (v.bytes + 255) & ~(size_t)255;
     touched_host = true;
+    return d;
+  }
+
+  // An output of which the call may write a part only: in host memory, the GPU
+  // copy that goes back starts as what the tensor holds.
+  void *inout(const View &v) {
+    const size_t before = backs.size();
+    void *d = out(v);
+    if (ok && backs.size() > before)
+      check(hipMemcpyAsync(d, v.data, v.bytes, hipMemcpyHostToDevice, c.stream),
+          "host-to-device copy");
     return d;
   }
 
@@ -2231,6 +2249,537 @@ void om_mi355x_DynQuantMatMulDequantLimits(OMTensor *y_t, OMTensor *ylim_t,
     int64_t activation) {
   dyn_quant_matmul_dequant("DynQuantMatMulDequantLimits", y_t, ylim_t, x_t,
       xlim_t, b_t, bzp_t, bscale_t, bias_t, activation);
+}
+
+} // extern "C"
+
+// ---------------------------------------------------------------------------
+// decoder layers in 8 and 4 bits
+// ---------------------------------------------------------------------------
+namespace {
+
+bool float_kind(const View &v, FloatKind &kind) {
+  switch (v.dtype) {
+  case OM_MI355X_TYPE_FLOAT:
+    kind = kF32;
+    return true;
+  case OM_MI355X_TYPE_FLOAT16:
+    kind = kF16;
+    return true;
+  case OM_MI355X_TYPE_BFLOAT16:
+    kind = kBF16;
+    return true;
+  default:
+    return false;
+  }
+}
+
+bool same_shape(const View &a, const View &b) {
+  if (a.rank != b.rank)
+    return false;
+  for (int64_t i = 0; i < a.rank; ++i)
+    if (a.shape[i] != b.shape[i])
+      return false;
+  return true;
+}
+
+// Sizes of single dimensions and numbers of blocks are held in 32 bits.
+constexpr int64_t kMostOfOne = (int64_t)1 << 30;
+constexpr int64_t kMostBlocks = ((int64_t)1 << 31) - 1;
+
+int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+// Heads as [B, H, S, D], or [B, S, H * D] (`heads` or `dim` given).
+struct Heads {
+  int64_t B = 0, S = 0, H = 0, D = 0;
+  bool heads_first = false;
+};
+bool heads_of(const View &v, int64_t heads, int64_t dim, const char *op,
+    const char *name, Heads &h) {
+  if (v.rank == 4) {
+    h = {v.shape[0], v.shape[2], v.shape[1], v.shape[3], true};
+    if ((heads > 0 && h.H != heads) || (dim > 0 && h.D != dim)) {
+      fail(EINVAL, "%s: %s is [.., %lld heads, .., %lld], which does not fit", op,
+          name, (long long)h.H, (long long)h.D);
+      return false;
+    }
+  } else if (v.rank == 3) {
+    const int64_t row = v.shape[2], by = dim > 0 ? dim : heads;
+    if (by <= 0 || row % by != 0 || (heads > 0 && dim > 0 && row != heads * dim)) {
+      fail(EINVAL, "%s: rows of %s (%lld elements) do not divide into heads", op,
+          name, (long long)row);
+      return false;
+    }
+    h = {v.shape[0], v.shape[1], dim > 0 ? row / dim : heads,
+        dim > 0 ? dim : row / heads, false};
+  } else {
+    fail(EINVAL, "%s: %s must be [B, H, S, D] or [B, S, H * D]", op, name);
+    return false;
+  }
+  if (h.B > kMostOfOne || h.S > kMostOfOne || h.H > kMostOfOne || h.D > kMostOfOne) {
+    fail(EINVAL, "%s: %s is too large", op, name);
+    return false;
+  }
+  return true;
+}
+
+// An optional i32 tensor of one entry a sequence.
+bool per_sequence(const OMTensor *t, int64_t B, const char *op, const char *name,
+    View &v) {
+  if (!t)
+    return true;
+  if (!view_of(t, name, v))
+    return false;
+  if (v.dtype != OM_MI355X_TYPE_INT32 || v.rank != 1 || v.shape[0] != B) {
+    fail(EINVAL, "%s: %s must be i32 [%lld]", op, name, (long long)B);
+    return false;
+  }
+  return true;
+}
+
+// The operands that describe a cache.
+struct CacheViews {
+  View kc, ks, vc, vs, table, past, counts;
+  bool has_table = false, has_counts = false;
+  int64_t pages = 0, H = 0, page_size = 0, D = 0, table_pages = 0;
+
+  bool read(const OMTensor *kc_t, const OMTensor *ks_t, const OMTensor *vc_t,
+      const OMTensor *vs_t, const char *op) {
+    if (!view_of(kc_t, "k_codes", kc) || !view_of(ks_t, "k_scales", ks) ||
+        !view_of(vc_t, "v_codes", vc) || !view_of(vs_t, "v_scales", vs))
+      return false;
+    if (kc.rank != 4 || kc.dtype != OM_MI355X_TYPE_UINT8 ||
+        vc.dtype != kc.dtype || !same_shape(kc, vc)) {
+      fail(EINVAL, "%s: codes must be ui8 [pages, H, page_size, D / 2], those of "
+                   "keys and values alike", op);
+      return false;
+    }
+    pages = kc.shape[0];
+    H = kc.shape[1];
+    page_size = kc.shape[2];
+    D = kc.shape[3] > 256 ? 0 : 2 * kc.shape[3];
+    if (!attention_head_ok((int)D)) {
+      fail(EINVAL, "%s: heads of %lld elements; 64, 96, 128, 192 and 256 are held",
+          op, (long long)(2 * kc.shape[3]));
+      return false;
+    }
+    if (ks.rank != 5 || ks.dtype != OM_MI355X_TYPE_FLOAT16 || vs.dtype != ks.dtype ||
+        !same_shape(ks, vs) || ks.shape[0] != pages || ks.shape[1] != H ||
+        ks.shape[2] != page_size || ks.shape[3] != D / kCacheGroup ||
+        ks.shape[4] != 2) {
+      fail(EINVAL, "%s: scales must be f16 [pages, H, page_size, %lld, 2]", op,
+          (long long)(D / kCacheGroup));
+      return false;
+    }
+    if (pages > kMostOfOne || H > kMostOfOne || page_size > kMostOfOne) {
+      fail(EINVAL, "%s: the cache's dimensions are too large", op);
+      return false;
+    }
+    return true;
+  }
+
+  // What says where the tokens of B sequences, S new ones of each, lie.
+  bool places(const OMTensor *table_t, const OMTensor *past_t,
+      const OMTensor *counts_t, int64_t B, int64_t S, const char *op) {
+    has_table = table_t != nullptr;
+    has_counts = counts_t != nullptr;
+    if (!past_t) {
+      fail(EINVAL, "%s: past is NULL", op);
+      return false;
+    }
+    if (!per_sequence(past_t, B, op, "past", past) ||
+        !per_sequence(counts_t, B, op, "counts", counts))
+      return false;
+    if (has_table) {
+      if (!view_of(table_t, "page_table", table))
+        return false;
+      if (table.dtype != OM_MI355X_TYPE_INT32 || table.rank != 2 || table.shape[0] != B) {
+        fail(EINVAL, "%s: page_table must be i32 [%lld, pages of a sequence]", op,
+            (long long)B);
+        return false;
+      }
+      table_pages = table.shape[1];
+      if (page_size % 16 != 0) {
+        fail(EINVAL, "%s: pages of %lld tokens; page_size must be a multiple of 16",
+            op, (long long)page_size);
+        return false;
+      }
+    } else if (pages < B) {
+      fail(EINVAL, "%s: %lld sequences without a page table, and %lld pages", op,
+          (long long)B, (long long)pages);
+      return false;
+    }
+    if (capacity() > kMostOfOne) {
+      fail(EINVAL, "%s: a sequence's pages hold more than 2^30 tokens", op);
+      return false;
+    }
+    return host_places_ok(B, S, op);
+  }
+  int64_t capacity() const { return has_table ? table_pages * page_size : page_size; }
+
+  // Host memory can be looked at: every token must have a place.
+  static bool readable(const View &v) {
+    return v.data && v.numel > 0 && !backed_lookup(v.data) && !is_device_ptr(v.data);
+  }
+  bool host_places_ok(int64_t B, int64_t S, const char *op) const {
+    const bool see_past = readable(past), see_counts = has_counts && readable(counts);
+    const bool see_table = has_table && readable(table);
+    for (int64_t b = 0; b < B; ++b) {
+      const int64_t n = see_counts ? ((const int32_t *)counts.data)[b] : S;
+      if (see_counts && (n < 0 || n > S)) {
+        fail(EINVAL, "%s: counts[%lld] is %lld, of %lld rows", op, (long long)b,
+            (long long)n, (long long)S);
+        return false;
+      }
+      if (!see_past)
+        continue;
+      const int64_t t = ((const int32_t *)past.data)[b];
+      if (t < 0 || (has_counts && !see_counts ? t : t + n) > capacity()) {
+        fail(EINVAL, "%s: past[%lld] is %lld, and the sequence's pages hold %lld "
+                     "tokens", op, (long long)b, (long long)t, (long long)capacity());
+        return false;
+      }
+      if (!see_table || (has_counts && !see_counts))
+        continue;
+      for (int64_t j = 0; j * page_size < t + n; ++j) {
+        const int64_t page = ((const int32_t *)table.data)[b * table_pages + j];
+        if (page < 0 || page >= pages) {
+          fail(EINVAL, "%s: page_table[%lld, %lld] is %lld, of %lld pages", op,
+              (long long)b, (long long)j, (long long)page, (long long)pages);
+          return false;
+        }
+      }
+    }
+    return true;
+  }
+
+  // On the GPU.  written: the codes and scales are outputs.
+  Cache4 on_gpu(Call &call, bool written) const {
+    auto cache = [&](const View &v) {
+      return written ? call.inout(v) : const_cast<void *>(call.in(v));
+    };
+    Cache4 c = {};
+    c.k_codes = (uint8_t *)cache(kc);
+    c.k_scales = (uint16_t *)cache(ks);
+    c.v_codes = (uint8_t *)cache(vc);
+    c.v_scales = (uint16_t *)cache(vs);
+    c.table = has_table ? (const int32_t *)call.in(table) : nullptr;
+    c.past = (const int32_t *)call.in(past);
+    c.counts = has_counts ? (const int32_t *)call.in(counts) : nullptr;
+    c.pages = pages;
+    c.page_size = page_size;
+    c.table_pages = table_pages;
+    c.H = (int)H;
+    c.D = (int)D;
+    return c;
+  }
+};
+
+} // namespace
+
+extern "C" {
+
+void om_mi355x_DynamicQuantizeBlocks(OMTensor *y_t, OMTensor *scale_t,
+    const OMTensor *x_t, int64_t block_rows) {
+  const char *const op = "DynamicQuantizeBlocks";
+  View y, sc, x;
+  if (!view_of(y_t, "y", y) || !view_of(scale_t, "y_scale", sc) ||
+      !view_of(x_t, "x", x))
+    return;
+  FloatKind kind;
+  if (!float_kind(x, kind) || y.dtype != OM_MI355X_TYPE_FLOAT8E4M3FN ||
+      x.rank < 1 || !same_shape(x, y) || sc.dtype != OM_MI355X_TYPE_FLOAT) {
+    fail(EINVAL, "%s: expected f32, f16 or bf16 x of at least one dimension, "
+                 "f8e4m3fn y of x's shape and f32 y_scale", op);
+    return;
+  }
+  if ((block_rows != 1 && block_rows != kBlock) || (block_rows == kBlock && x.rank != 2)) {
+    fail(EINVAL, "%s: block_rows must be 1, or 128 with a 2-D x", op);
+    return;
+  }
+  const int64_t K = x.shape[x.rank - 1], M = K > 0 ? x.numel / K : 0;
+  const int64_t scales = (M + block_rows - 1) / block_rows * blocks_of(K);
+  if (sc.numel != scales) {
+    fail(EINVAL, "%s: y_scale has %lld entries, expected %lld", op,
+        (long long)sc.numel, (long long)scales);
+    return;
+  }
+  if (K > kMostOfOne || scales > kMostBlocks) {
+    fail(EINVAL, "%s: x is too large", op);
+    return;
+  }
+  if (x.numel == 0)
+    return;
+  Call call(t_ctx, op);
+  if (!call.ok)
+    return;
+  uint8_t *const dy = (uint8_t *)call.out(y);
+  float *const ds = (float *)call.out(sc);
+  const void *const dx = call.in(x);
+  if (call.ok)
+    call.check(launch_quantize_blocks(
+                   call.c.stream, dx, kind, M, K, (int)block_rows, dy, ds),
+        op);
+  call.finish();
+}
+
+void om_mi355x_MatMulBlocks(OMTensor *y_t, const OMTensor *a_t,
+    const OMTensor *a_scale_t, const OMTensor *b_t, const OMTensor *b_scale_t,
+    const OMTensor *bias_t, int64_t activation) {
+  const char *const op = "MatMulBlocks";
+  View y, a, as, b, bs, bias;
+  if (!view_of(y_t, "y", y) || !view_of(a_t, "a", a) ||
+      !view_of(a_scale_t, "a_scale", as) || !view_of(b_t, "b", b) ||
+      !view_of(b_scale_t, "b_scale", bs))
+    return;
+  BlockGemm g = {};
+  if (!float_kind(y, g.kind) || a.dtype != OM_MI355X_TYPE_FLOAT8E4M3FN ||
+      b.dtype != a.dtype || a.rank < 1 || b.rank != 2) {
+    fail(EINVAL, "%s: expected f8e4m3fn a [.., K] and b [N, K], and f32, f16 or "
+                 "bf16 y", op);
+    return;
+  }
+  g.K = a.shape[a.rank - 1];
+  g.N = b.shape[0];
+  g.M = 1;
+  for (int64_t i = 0; i + 1 < a.rank; ++i)
+    g.M *= a.shape[i];
+  if (b.shape[1] != g.K) {
+    fail(EINVAL, "%s: inner dimensions differ (%lld vs %lld)", op, (long long)g.K,
+        (long long)b.shape[1]);
+    return;
+  }
+  if (y.numel != g.M * g.N || y.rank < 1 || y.shape[y.rank - 1] != g.N) {
+    fail(EINVAL, "%s: output has %lld elements, expected %lld in rows of %lld", op,
+        (long long)y.numel, (long long)(g.M * g.N), (long long)g.N);
+    return;
+  }
+  if (as.dtype != OM_MI355X_TYPE_FLOAT || bs.dtype != OM_MI355X_TYPE_FLOAT ||
+      as.numel != g.M * blocks_of(g.K) ||
+      bs.numel != blocks_of(g.N) * blocks_of(g.K)) {
+    fail(EINVAL, "%s: scales must be f32, a_scale [.., %lld] and b_scale "
+                 "[%lld, %lld]", op, (long long)blocks_of(g.K),
+        (long long)blocks_of(g.N), (long long)blocks_of(g.K));
+    return;
+  }
+  if (!bias_ok(bias_t, g.N, op, bias))
+    return;
+  bool relu, gelu;
+  if (!activation_ok(activation, op, relu, gelu))
+    return;
+  if (g.M > kMostOfOne || g.N > kMostOfOne || g.K > kMostOfOne ||
+      blocks_of(g.M) * blocks_of(g.N) > kMostBlocks) {
+    fail(EINVAL, "%s: the product is too large", op);
+    return;
+  }
+  if (g.M == 0 || g.N == 0)
+    return;
+  Call call(t_ctx, op);
+  if (!call.ok)
+    return;
+  g.y = call.out(y);
+  g.a = (const uint8_t *)call.in(a);
+  g.a_scale = (const float *)call.in(as);
+  g.b = (const uint8_t *)call.in(b);
+  g.b_scale = (const float *)call.in(bs);
+  if (bias_t) {
+    g.bias = (const float *)call.in(bias);
+    g.bias_len = bias.numel;
+  }
+  g.activation = (int)activation;
+  void *scratch = nullptr;
+  if (call.ok)
+    if (const size_t bytes = block_gemm_scratch(g))
+      scratch = call.temp(bytes);
+  if (call.ok)
+    call.check(launch_block_gemm(call.c.stream, g, scratch), op);
+  call.finish();
+}
+
+void om_mi355x_RotaryEmbedding(OMTensor *y_t, const OMTensor *x_t,
+    const OMTensor *cos_t, const OMTensor *sin_t, const OMTensor *position_t,
+    int64_t interleaved, int64_t num_heads, int64_t rotary_embedding_dim) {
+  const char *const op = "RotaryEmbedding";
+  View y, x, cs, sn, pos;
+  if (!view_of(y_t, "y", y) || !view_of(x_t, "x", x) ||
+      !view_of(cos_t, "cos_cache", cs) || !view_of(sin_t, "sin_cache", sn))
+    return;
+  Rotary r = {};
+  if (!float_kind(x, r.kind) || y.dtype != x.dtype || !same_shape(x, y)) {
+    fail(EINVAL, "%s: expected f32, f16 or bf16 x and y of x's type and shape", op);
+    return;
+  }
+  if (num_heads < 0 || interleaved < 0 || interleaved > 1) {
+    fail(EINVAL, "%s: num_heads must not be negative, interleaved 0 or 1", op);
+    return;
+  }
+  Heads h;
+  if (!heads_of(x, num_heads, 0, op, "x", h))
+    return;
+  const int64_t rot = rotary_embedding_dim ? rotary_embedding_dim : h.D;
+  if (rot < 0 || rot > h.D || rot % 2 != 0) {
+    fail(EINVAL, "%s: %lld elements of heads of %lld cannot be rotated", op,
+        (long long)rot, (long long)h.D);
+    return;
+  }
+  if (cs.dtype != OM_MI355X_TYPE_FLOAT || sn.dtype != cs.dtype ||
+      !same_shape(cs, sn) || cs.rank != (position_t ? 2 : 3) ||
+      cs.shape[cs.rank - 1] != rot / 2 ||
+      (!position_t && (cs.shape[0] != h.B || cs.shape[1] != h.S))) {
+    fail(EINVAL, "%s: tables must be f32 [positions, %lld] with position_ids, "
+                 "[B, S, %lld] without", op, (long long)(rot / 2), (long long)(rot / 2));
+    return;
+  }
+  if (position_t) {
+    if (!view_of(position_t, "position_ids", pos))
+      return;
+    if (pos.dtype != OM_MI355X_TYPE_INT64 || pos.rank != 2 || pos.shape[0] != h.B ||
+        pos.shape[1] != h.S) {
+      fail(EINVAL, "%s: position_ids must be i64 [%lld, %lld]", op, (long long)h.B,
+          (long long)h.S);
+      return;
+    }
+  }
+  if ((x.numel + 511) / 512 > kMostBlocks) {
+    fail(EINVAL, "%s: x is too large", op);
+    return;
+  }
+  if (x.numel == 0)
+    return;
+  Call call(t_ctx, op);
+  if (!call.ok)
+    return;
+  r.y = call.out(y);
+  r.x = call.in(x);
+  r.cos = (const float *)call.in(cs);
+  r.sin = (const float *)call.in(sn);
+  r.positions = position_t ? (const int64_t *)call.in(pos) : nullptr;
+  r.table_rows = position_t ? cs.shape[0] : h.B * h.S;
+  r.B = h.B;
+  r.S = h.S;
+  r.H = h.H;
+  r.D = (int)h.D;
+  r.rot = (int)rot;
+  r.interleaved = interleaved != 0;
+  r.heads_first = h.heads_first;
+  if (call.ok)
+    call.check(launch_rotary(call.c.stream, r), op);
+  call.finish();
+}
+
+void om_mi355x_CacheAppend4(OMTensor *k_codes, OMTensor *k_scales,
+    OMTensor *v_codes, OMTensor *v_scales, const OMTensor *k_t,
+    const OMTensor *v_t, const OMTensor *page_table, const OMTensor *past,
+    const OMTensor *counts) {
+  const char *const op = "CacheAppend4";
+  CacheViews cache;
+  View k, v;
+  if (!cache.read(k_codes, k_scales, v_codes, v_scales, op) ||
+      !view_of(k_t, "k", k) || !view_of(v_t, "v", v))
+    return;
+  Append4 a = {};
+  if (!float_kind(k, a.kind) || v.dtype != k.dtype || !same_shape(k, v)) {
+    fail(EINVAL, "%s: expected f32, f16 or bf16 k, and v of k's type and shape", op);
+    return;
+  }
+  Heads h;
+  if (!heads_of(k, cache.H, cache.D, op, "k", h) ||
+      !cache.places(page_table, past, counts, h.B, h.S, op))
+    return;
+  if (k.numel / 64 > kMostBlocks) {
+    fail(EINVAL, "%s: k is too large", op);
+    return;
+  }
+  if (k.numel == 0)
+    return;
+  Call call(t_ctx, op);
+  if (!call.ok)
+    return;
+  a.c = cache.on_gpu(call, /*written=*/true);
+  a.k = call.in(k);
+  a.v = call.in(v);
+  a.B = h.B;
+  a.S = h.S;
+  a.heads_first = h.heads_first;
+  if (call.ok && a.c.page_size > 0 && a.c.pages > 0)
+    call.check(launch_cache_append(call.c.stream, a), op);
+  call.finish();
+}
+
+void om_mi355x_CacheAttention4(OMTensor *y_t, const OMTensor *q_t,
+    const OMTensor *k_codes, const OMTensor *k_scales,
+    const OMTensor *v_codes, const OMTensor *v_scales,
+    const OMTensor *page_table, const OMTensor *past, const OMTensor *counts,
+    const OMTensor *starts_t, const OMTensor *scale_t, int64_t causal,
+    int64_t window) {
+  const char *const op = "CacheAttention4";
+  CacheViews cache;
+  View y, q, starts, scale;
+  if (!view_of(y_t, "y", y) || !view_of(q_t, "q", q) ||
+      !cache.read(k_codes, k_scales, v_codes, v_scales, op))
+    return;
+  Attention4 a = {};
+  if (!float_kind(q, a.kind) || y.dtype != q.dtype || !same_shape(q, y)) {
+    fail(EINVAL, "%s: expected f32, f16 or bf16 q, and y of q's type and shape", op);
+    return;
+  }
+  if (causal < 0 || causal > 1 || window < 0) {
+    fail(EINVAL, "%s: causal must be 0 or 1, window not negative", op);
+    return;
+  }
+  Heads h;
+  if (!heads_of(q, 0, cache.D, op, "q", h) ||
+      !cache.places(page_table, past, counts, h.B, h.S, op) ||
+      !per_sequence(starts_t, h.B, op, "starts", starts))
+    return;
+  if (scale_t) {
+    if (!view_of(scale_t, "scale", scale))
+      return;
+    if (scale.dtype != OM_MI355X_TYPE_FLOAT || scale.numel != 1) {
+      fail(EINVAL, "%s: scale must be an f32 scalar", op);
+      return;
+    }
+  }
+  if (q.numel == 0)
+    return;
+  if (cache.H == 0 || h.H % cache.H != 0) {
+    fail(EINVAL, "%s: %lld query heads on %lld heads of keys", op, (long long)h.H,
+        (long long)cache.H);
+    return;
+  }
+  if (cache.pages == 0 || cache.capacity() == 0) {
+    fail(EINVAL, "%s: the cache has no room", op);
+    return;
+  }
+  a.B = h.B;
+  a.S = h.S;
+  a.heads = h.H;
+  a.window = window;
+  a.causal = causal != 0;
+  a.heads_first = h.heads_first;
+  if (h.H > kMostOfOne / h.S || h.B * cache.H > kMostOfOne / 256 ||
+      h.B * cache.H > kMostBlocks / 256 / (h.S * (h.H / cache.H) / 16 + 1)) {
+    fail(EINVAL, "%s: q is too large", op);
+    return;
+  }
+  Call call(t_ctx, op);
+  if (!call.ok)
+    return;
+  // (rows that are not queries stay as they are)
+  a.y = counts ? call.inout(y) : call.out(y);
+  a.q = call.in(q);
+  a.c = cache.on_gpu(call, /*written=*/false);
+  a.starts = starts_t ? (const int32_t *)call.in(starts) : nullptr;
+  a.scale = scale_t ? (const float *)call.in(scale) : nullptr;
+  a.splits = 1;
+  if (call.ok) {
+    a.splits = attention_splits(a);
+    // (without room for the parts: in one piece)
+    if (a.splits > 1 && !(a.parts = (float *)call.scratch_for(attention_parts_bytes(a))))
+      a.splits = 1;
+    call.check(launch_cache_attention(call.c.stream, a), op);
+  }
+  call.finish();
 }
 
 // ---------------------------------------------------------------------------

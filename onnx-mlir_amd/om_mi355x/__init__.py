@@ -6,7 +6,9 @@ QLinearMatMul; src/Conversion/ONNXToKrnl/ConvertONNXToKrnl.cpp:226-241) and
 call the C-ABI entry points of ``include/om_mi355x.h`` exactly as a compiled
 model's ``krnl.call`` would: outputs first, then inputs, then integer
 attributes, every tensor wrapped in an ``OMTensor``
-(src/Conversion/KrnlToLLVM/KrnlCall.cpp:34-102).
+(src/Conversion/KrnlToLLVM/KrnlCall.cpp:34-102).  Beside them stand the ops of
+decoder layers held in 8 and 4 bits (DynamicQuantizeBlocks, MatMulBlocks,
+RotaryEmbedding, CacheAppend4, CacheAttention4), called the same way.
 
 Operands may be numpy arrays (host memory: the runtime stages them through the
 GPU and copies results back) or :class:`DeviceArray` (GPU memory owned by the
@@ -32,11 +34,22 @@ MEASURE_PATH = os.path.join(_CSRC, "libom_mi355x_measure.so")
 
 # ONNX element-type codes (include/onnx-mlir/Runtime/OnnxDataTypeMetaData.inc:22-44)
 ONNX_FLOAT, ONNX_UINT8, ONNX_INT8, ONNX_INT32 = 1, 2, 3, 6
+ONNX_INT64, ONNX_FLOAT16, ONNX_BFLOAT16, ONNX_FLOAT8E4M3FN = 7, 10, 16, 17
+
+# Element types that numpy does not have: an array of such a dtype holds the
+# bits, ``a["bits"]`` gives them (see from_float32, to_float32).
+bfloat16 = np.dtype([("bits", np.uint16)], metadata={"name": "bfloat16"})
+float8_e4m3fn = np.dtype([("bits", np.uint8)], metadata={"name": "float8_e4m3fn"})
+
 _NP_TO_ONNX = {
     np.dtype(np.float32): ONNX_FLOAT,
     np.dtype(np.uint8): ONNX_UINT8,
     np.dtype(np.int8): ONNX_INT8,
     np.dtype(np.int32): ONNX_INT32,
+    np.dtype(np.int64): ONNX_INT64,
+    np.dtype(np.float16): ONNX_FLOAT16,
+    bfloat16: ONNX_BFLOAT16,
+    float8_e4m3fn: ONNX_FLOAT8E4M3FN,
 }
 
 WRAP, SATURATE = 0, 1
@@ -46,7 +59,7 @@ ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_GELU = 0, 1, 2
 # --enable-fast-math and --disable-quantization-zero-point
 QUANT_RECIPROCAL, QUANT_NO_ZERO_POINT = 1, 2
 # OM_MI355X_VERSION of the header this module was written against
-VERSION = 0x00010100
+VERSION = 0x00010200
 
 
 class RuntimeError_(RuntimeError):
@@ -95,6 +108,11 @@ def _declare(lib, shim):
         "om_mi355x_QLinearMatMul": [P, P, P, P, P, P, P, P, P, I64],
         "om_mi355x_DynQuantMatMulDequant": [P, P, P, P, P, P, I64],
         "om_mi355x_DynQuantMatMulDequantLimits": [P, P, P, P, P, P, P, P, I64],
+        "om_mi355x_DynamicQuantizeBlocks": [P, P, P, I64],
+        "om_mi355x_MatMulBlocks": [P, P, P, P, P, P, I64],
+        "om_mi355x_RotaryEmbedding": [P, P, P, P, P, I64, I64, I64],
+        "om_mi355x_CacheAppend4": [P, P, P, P, P, P, P, P, P],
+        "om_mi355x_CacheAttention4": [P, P, P, P, P, P, P, P, P, P, P, I64, I64],
         "om_mi355x_MarkConstant": [P],
         "om_mi355x_UnmarkConstant": [P],
         "om_mi355x_KeepOnDevice": [P],
@@ -251,6 +269,22 @@ class DeviceArray:
         assert offset_elems * v.dtype.itemsize + v.nbytes <= owner.nbytes
         v.ptr = owner.ptr + offset_elems * v.dtype.itemsize
         v.owner = owner
+        return v
+
+    @classmethod
+    def wrap(cls, ptr: int, shape, dtype, owner=None) -> "DeviceArray":
+        """GPU memory that something else allocated, as a row-major tensor.
+        ``owner`` is kept alive with it; ``free`` leaves the memory alone.  The
+        ops run on the runtime's own stream: what fills or reads the memory on
+        another one has to be ordered with them (``synchronize``)."""
+        load()
+        v = cls.__new__(cls)
+        v.shape = tuple(int(s) for s in shape)
+        v.dtype = np.dtype(dtype)
+        v.size = int(np.prod(v.shape, dtype=np.int64)) if v.shape else 1
+        v.nbytes = v.size * v.dtype.itemsize
+        v.ptr = int(ptr)
+        v.owner = owner if owner is not None else ()
         return v
 
     def numpy(self) -> np.ndarray:
@@ -545,6 +579,191 @@ def DynQuantMatMulDequantLimits(x: Tensor, b: Tensor, b_zero_point: Optional[Ten
         _lib.om_mi355x_DynQuantMatMulDequantLimits(hy, hyl, hx, hxl, hb, hbz, hbs, hbias, int(activation))
     _check()
     return y, yl
+
+
+# ---- decoder layers in 8 and 4 bits -------------------------------------------
+BLOCK = 128          # elements of a row under one scale (DynamicQuantizeBlocks)
+CACHE_GROUP = 32     # elements under one scale and lowest value (the 4-bit cache)
+
+
+def from_float32(x, dtype) -> np.ndarray:
+    """Host array of ``x`` in ``dtype`` (float32, float16 or bfloat16), rounded to
+    nearest even."""
+    x = np.ascontiguousarray(x, np.float32)
+    if np.dtype(dtype) != bfloat16:
+        return x.astype(dtype)
+    u = x.view(np.uint32)
+    bits = ((u + (0x7FFF + ((u >> 16) & 1))) >> 16).astype(np.uint16)
+    bits = np.where(np.isnan(x), np.uint16(0x7FC0), bits)
+    return np.ascontiguousarray(bits).view(bfloat16).reshape(x.shape)
+
+
+def to_float32(a: np.ndarray) -> np.ndarray:
+    """The values of a host array of any of the runtime's floating types."""
+    if a.dtype == bfloat16:
+        return (a["bits"].astype(np.uint32) << 16).view(np.float32)
+    if a.dtype == float8_e4m3fn:
+        return _E4M3_VALUES[a["bits"]]
+    return a.astype(np.float32)
+
+
+def _e4m3_values() -> np.ndarray:
+    code = np.arange(256)
+    e, m = (code >> 3) & 15, code & 7
+    v = np.where(e > 0, np.ldexp(8.0 + m, e - 10), np.ldexp(m.astype(np.float64), -9))
+    v = np.where((code & 127) == 127, np.nan, v)
+    return np.where(code & 128, -v, v).astype(np.float32)
+
+
+_E4M3_VALUES = _e4m3_values()
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def DynamicQuantizeBlocks(x: Tensor, block_rows: int = 1,
+                          out: Optional[Tuple[Tensor, Tensor]] = None) -> Tuple[Tensor, Tensor]:
+    """om_mi355x_DynamicQuantizeBlocks: (y, y_scale) of a float32, float16 or
+    bfloat16 tensor, with a scale for each 128 neighbouring elements of a row, or
+    (``block_rows`` = 128, a matrix) for each block of 128 x 128."""
+    load()
+    x = _host(x)
+    if out is not None:
+        y, s = out
+    else:
+        k = x.shape[-1] if len(x.shape) else 0
+        y = _like(x, x.shape, float8_e4m3fn)
+        s = _like(x, tuple(x.shape[:-1]) + (_blocks(k),) if block_rows == 1 else
+                  (_blocks(x.shape[0]) if len(x.shape) else 0, _blocks(k)), np.float32)
+    with _OMT(y) as hy, _OMT(s) as hs, _OMT(x) as hx:
+        _lib.om_mi355x_DynamicQuantizeBlocks(hy, hs, hx, int(block_rows))
+    _check()
+    return y, s
+
+
+def MatMulBlocks(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Optional[Tensor] = None,
+                 activation: int = ACTIVATION_NONE, dtype=np.float32, out: Optional[Tensor] = None) -> Tensor:
+    """om_mi355x_MatMulBlocks: ``a`` [.., K] times ``b`` [N, K] transposed, both e4m3
+    with the scales of DynamicQuantizeBlocks (``b``: block_rows = 128); the result
+    has ``dtype`` (float32, float16 or bfloat16)."""
+    load()
+    a, b, a_scale, b_scale = _host(a), _host(b), _host(a_scale, np.float32), _host(b_scale, np.float32)
+    bias = None if bias is None else _host(bias, np.float32)
+    y = out if out is not None else _like(a, tuple(a.shape[:-1]) + (b.shape[0],), dtype)
+    with _OMT(y) as hy, _OMT(a) as ha, _OMT(a_scale) as has, _OMT(b) as hb, _OMT(b_scale) as hbs, \
+            _OMT(bias) as hbias:
+        _lib.om_mi355x_MatMulBlocks(hy, ha, has, hb, hbs, hbias, int(activation))
+    _check()
+    return y
+
+
+def rotary_tables(positions: int, dim: int, base: float = 10000.0, scaling: Optional[str] = None,
+                  factor: float = 1.0, trained: int = 0) -> Tuple[np.ndarray, np.ndarray]:
+    """(cos, sin), float32 [positions, dim / 2], of the angles p * base^(-2 i / dim),
+    computed in 64 bits, for RotaryEmbedding.  ``scaling``, for contexts ``factor``
+    times as long as the model was trained on:
+      None      as they are
+      "linear"  positions divided by ``factor``
+      "ntk"     base * factor^(dim / (dim - 2)): the lowest rate divided by
+                ``factor``, the highest left alone
+      "yarn"    rates that turn less than once within ``trained`` positions are
+                divided by ``factor``, those that turn more than 32 times left
+                alone, those between interpolated (Peng et al. 2023, "YaRN"); cos
+                and sin times 0.1 ln(factor) + 1, that paper's temperature."""
+    if dim < 2 or dim % 2 or positions < 0 or factor < 1.0:
+        raise ValueError("rotary_tables: dim must be even and positive, factor at least 1")
+    i = np.arange(0, dim, 2, dtype=np.float64)
+    gain = 1.0
+    if scaling == "ntk":
+        if dim < 4:
+            raise ValueError("rotary_tables: ntk scaling needs a dim of at least 4")
+        base = base * factor ** (dim / (dim - 2))
+    rate = base ** (-i / dim)
+    if scaling == "linear":
+        rate = rate / factor
+    elif scaling == "yarn":
+        if trained <= 0:
+            raise ValueError("rotary_tables: yarn scaling needs the trained length")
+        keep = np.clip((trained * rate / (2 * np.pi) - 1.0) / (32.0 - 1.0), 0.0, 1.0)
+        rate = keep * rate + (1.0 - keep) * rate / factor
+        gain = 0.1 * np.log(factor) + 1.0
+    elif scaling not in (None, "ntk"):
+        raise ValueError(f"rotary_tables: unknown scaling {scaling!r}")
+    angle = np.arange(positions, dtype=np.float64)[:, None] * rate
+    return (gain * np.cos(angle)).astype(np.float32), (gain * np.sin(angle)).astype(np.float32)
+
+
+def RotaryEmbedding(x: Tensor, cos_cache: Tensor, sin_cache: Tensor, position_ids: Optional[Tensor] = None,
+                    interleaved: int = 0, num_heads: int = 0, rotary_embedding_dim: int = 0,
+                    out: Optional[Tensor] = None) -> Tensor:
+    """onnx.RotaryEmbedding: ``x`` [B, H, S, D], or [B, S, H * D] with ``num_heads``;
+    tables of rotary_tables with ``position_ids`` int64 [B, S], or tables
+    [B, S, rotary_embedding_dim / 2].  ``out`` may be ``x``."""
+    load()
+    x, cos_cache, sin_cache = _host(x), _host(cos_cache, np.float32), _host(sin_cache, np.float32)
+    pos = None if position_ids is None else _host(position_ids, np.int64)
+    y = out if out is not None else _like(x, x.shape, x.dtype)
+    with _OMT(y) as hy, _OMT(x) as hx, _OMT(cos_cache) as hc, _OMT(sin_cache) as hs, _OMT(pos) as hp:
+        _lib.om_mi355x_RotaryEmbedding(hy, hx, hc, hs, hp, int(interleaved), int(num_heads),
+                                       int(rotary_embedding_dim))
+    _check()
+    return y
+
+
+class Cache4:
+    """The 4-bit cache of keys and values of one layer: the tensors that
+    CacheAppend4 writes and CacheAttention4 reads (include/om_mi355x.h says how
+    they hold a row).  ``template`` says where they live: a DeviceArray for GPU
+    memory, anything else for numpy arrays."""
+
+    def __init__(self, pages: int, heads: int, page_size: int, head_size: int, template: Optional[Tensor] = None):
+        lead = (int(pages), int(heads), int(page_size))
+        groups = int(head_size) // CACHE_GROUP
+        shapes = [(lead + (int(head_size) // 2,), np.uint8), (lead + (groups, 2), np.float16)] * 2
+        if isinstance(template, DeviceArray):
+            arrays = [DeviceArray.from_numpy(np.zeros(s, d)) for s, d in shapes]
+        else:
+            arrays = [np.zeros(s, d) for s, d in shapes]
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = arrays
+
+    @property
+    def tensors(self):
+        return self.k_codes, self.k_scales, self.v_codes, self.v_scales
+
+
+def CacheAppend4(cache: Cache4, k: Tensor, v: Tensor, past: Tensor, page_table: Optional[Tensor] = None,
+                 counts: Optional[Tensor] = None) -> Cache4:
+    """om_mi355x_CacheAppend4: stores the new tokens' keys and values in ``cache``."""
+    load()
+    k, v = _host(k), _host(v)
+    past, table, counts = (None if t is None else _host(t, np.int32) for t in (past, page_table, counts))
+    kc, ks, vc, vs = cache.tensors
+    with _OMT(kc) as hkc, _OMT(ks) as hks, _OMT(vc) as hvc, _OMT(vs) as hvs, _OMT(k) as hk, _OMT(v) as hv, \
+            _OMT(table) as ht, _OMT(past) as hp, _OMT(counts) as hn:
+        _lib.om_mi355x_CacheAppend4(hkc, hks, hvc, hvs, hk, hv, ht, hp, hn)
+    _check()
+    return cache
+
+
+def CacheAttention4(q: Tensor, cache: Cache4, past: Tensor, page_table: Optional[Tensor] = None,
+                    counts: Optional[Tensor] = None, starts: Optional[Tensor] = None,
+                    scale: Optional[Tensor] = None, causal: int = 1, window: int = 0,
+                    out: Optional[Tensor] = None) -> Tensor:
+    """om_mi355x_CacheAttention4: attention of the new tokens' queries over ``cache``,
+    which holds their keys and values already.  With ``counts``, give ``out`` to
+    say what the rows behind a sequence's tokens hold."""
+    load()
+    q = _host(q)
+    past, table, counts, starts = (None if t is None else _host(t, np.int32) for t in (past, page_table, counts, starts))
+    scale = None if scale is None else _host(scale, np.float32)
+    y = out if out is not None else _like(q, q.shape, q.dtype)
+    kc, ks, vc, vs = cache.tensors
+    with _OMT(y) as hy, _OMT(q) as hq, _OMT(kc) as hkc, _OMT(ks) as hks, _OMT(vc) as hvc, _OMT(vs) as hvs, \
+            _OMT(table) as ht, _OMT(past) as hp, _OMT(counts) as hn, _OMT(starts) as hst, _OMT(scale) as hsc:
+        _lib.om_mi355x_CacheAttention4(hy, hq, hkc, hks, hvc, hvs, ht, hp, hn, hst, hsc, int(causal), int(window))
+    _check()
+    return y
 
 
 class PreparedCall:

@@ -1,0 +1,569 @@
+"""Block quantization, block-scaled products, rotary positions, the 4-bit cache and
+attention over it, against tests/blocks_reference.py.
+
+Tolerances.  A result's last rounding is at most half a step of its type.  Before
+it, f32 sums of n terms are off by at most n 2^-24 of the sum of their magnitudes,
+whatever their order; products of e4m3 values, and of codes 0 .. 15 with bf16
+terms, are exact in f32.  The matrix instructions for 8-bit operands, which
+results of 16 bits and more than 64 rows take, align the products of a block to
+its largest: 2^-12 of the sum of their magnitudes covers what they drop."""
+import numpy as np
+import pytest
+
+import blocks_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["f32", "f16", "bf16"]
+
+
+@pytest.fixture(scope="module")
+def om():
+    import om_mi355x
+    om_mi355x.load()
+    return om_mi355x
+
+
+def dt(om, name):
+    return {"f32": np.dtype(np.float32), "f16": np.dtype(np.float16), "bf16": om.bfloat16}[name]
+
+
+def on(om, a):
+    return om.DeviceArray.from_numpy(a)
+
+
+def back(om, a):
+    return om.to_float32(a.numpy() if isinstance(a, om.DeviceArray) else a)
+
+
+def bits(a):
+    return np.ascontiguousarray(a).view(np.uint8)
+
+
+def equal(a, b):
+    """Equal, NaN in the same places."""
+    return a.shape == b.shape and np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(np.nan_to_num(a), np.nan_to_num(b))
+
+
+# ---------------------------------------------------------------------------
+# quantization
+# ---------------------------------------------------------------------------
+def awkward(rng, shape):
+    """Values of many magnitudes, exact ties among them, and blocks of zeros."""
+    x = rng.standard_normal(shape).astype(np.float32) * np.exp2(rng.integers(-6, 7, shape)).astype(np.float32)
+    x[rng.random(shape) < 0.05] = 0
+    return x
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 128])
+@pytest.mark.parametrize("shape", [(1, 1), (1, 128), (3, 127), (2, 129), (5, 776), (37, 777), (129, 384), (130, 264), (300, 8), (64, 4096)])
+def test_quantize_blocks(om, shape, rows, dtype):
+    rng = np.random.default_rng(sum(shape) + rows)
+    x = om.from_float32(awkward(rng, shape), dt(om, dtype))
+    y, s = om.DynamicQuantizeBlocks(on(om, x), rows)
+    want, ws = ref.quantize_blocks(om.to_float32(x), rows)
+    assert np.array_equal(s.numpy(), ws)
+    assert np.array_equal(y.numpy()["bits"], want)
+
+
+def test_quantize_blocks_where_rounding_is_decided(om):
+    """Quotients on, and next to, every border between two codes, for scales of
+    many magnitudes, those too small or large for the short form of the divide
+    among them."""
+    codes = np.arange(126)
+    v = np.where(codes >> 3 > 0, np.ldexp(8.0 + (codes & 7), (codes >> 3) - 10), np.ldexp(codes * 1.0, -9))
+    middle = ((v[:-1] + v[1:]) / 2).astype(np.float32)
+    rows = []
+    for power in (-149, -140, -120, -100, -85, -79, -30, -3, 0, 5, 60, 90, 97, 110, 118):
+        for top in (448.0, 447.0, 301.7, 255.99):
+            amax = np.float32(np.ldexp(top, power))
+            if not np.isfinite(amax) or amax == 0:
+                continue
+            s = np.float32(max(np.float32(amax / np.float32(448)), np.float32(2.0 ** -126)))
+            x = (middle.astype(np.float64) * s).astype(np.float32)
+            for y in (x, np.nextafter(x, np.float32(np.inf)), -np.nextafter(x, np.float32(0))):
+                y = np.where(np.abs(y) > amax, 0, y).astype(np.float32)
+                rows.append(np.concatenate([[amax], y, [0, 0]]).astype(np.float32))
+    x = np.stack(rows)
+    assert x.shape[1] == 128
+    y, s = om.DynamicQuantizeBlocks(on(om, x))
+    want, ws = ref.quantize_blocks(x, 1)
+    assert np.array_equal(s.numpy(), ws)
+    assert np.array_equal(y.numpy()["bits"], want)
+
+
+def test_quantize_blocks_of_zeros_infinities_and_nan(om):
+    x = np.zeros((6, 256), np.float32)
+    x[1, 3] = np.nan
+    x[2, 200] = np.inf
+    x[3, :128] = np.nan
+    x[4, 5], x[4, 6], x[4, 7] = np.nan, -2.0, 1.0
+    x[5, 0], x[5, 1] = -np.inf, 3.0
+    y, s = om.DynamicQuantizeBlocks(on(om, x))
+    v = back(om, y)
+    s = s.numpy()
+    assert s[0, 0] == s[0, 1] == s[1, 0] == s[3, 0] == np.float32(2.0 ** -126) and not v[0].any()
+    assert np.isnan(v[1, 3]) and not np.delete(v[1], 3).any()
+    assert np.isinf(s[2, 1]) and np.isnan(v[2, 200]) and not v[2, 128:200].any() and s[2, 0] == s[0, 0]
+    assert np.isnan(v[3, :128]).all() and not v[3, 128:].any()
+    assert np.isnan(v[4, 5]) and v[4, 6] == -448 and v[4, 7] == 224
+    assert np.isnan(v[5, 0]) and v[5, 1] == 0 and np.isinf(s[5, 0])
+
+
+@pytest.mark.parametrize("shape", [(0, 128), (3, 0)])
+def test_quantize_nothing(om, shape):
+    y, s = om.DynamicQuantizeBlocks(on(om, np.zeros(shape, np.float32)))
+    assert y.numpy().shape == shape and s.numpy().size == 0
+
+
+def test_quantize_rows_of_any_address_and_leading_dimensions(om):
+    """A window that starts 4 bytes into memory: rows that no wide load can take."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal(1 + 2 * 3 * 136).astype(np.float32)
+    d = on(om, x)
+    y, s = om.DynamicQuantizeBlocks(om.DeviceArray.view_of(d, 1, (2, 3, 136)))
+    want, ws = ref.quantize_blocks(x[1:].reshape(6, 136), 1)
+    assert y.shape == (2, 3, 136) and s.shape == (2, 3, 2)
+    assert np.array_equal(y.numpy()["bits"].reshape(6, 136), want) and np.array_equal(s.numpy().reshape(6, 2), ws)
+
+
+# ---------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------
+def operands(om, rng, M, K, N):
+    a, sa = ref.quantize_blocks((rng.standard_normal((M, K)) * np.where(rng.random(K) < 0.02, 16, 1)).astype(np.float32), 1)
+    b, sb = ref.quantize_blocks((0.02 * rng.standard_normal((N, K))).astype(np.float32), 128)
+    return a.view(om.float8_e4m3fn), sa, b.view(om.float8_e4m3fn), sb
+
+
+def product(om, a, sa, b, sb, bias=None, act=0):
+    """The result and the sum of its terms' magnitudes, in 64 bits."""
+    (M, K), N = a.shape, b.shape[0]
+    x = om.to_float32(a).astype(np.float64) * ref.spread(sa, 1, M, K)
+    w = om.to_float32(b).astype(np.float64) * ref.spread(sb, 128, N, K)
+    y, size = x @ w.T, np.abs(x) @ np.abs(w).T
+    if bias is not None:
+        y, size = y + bias.astype(np.float64), size + np.abs(bias.astype(np.float64))
+    if act == om.ACTIVATION_RELU:
+        y = np.maximum(y, 0)
+    elif act == om.ACTIVATION_GELU:
+        from scipy.special import ndtr
+        y = y * ndtr(y)
+    return y, size
+
+
+def check_product(om, got, want, size, dtype, rows, K):
+    # sums: 128 terms of a block, a scale and a sum for every block, the bias;
+    # Gelu: its slope is below 1.13, its own error below 2^-21 of its argument
+    off = (128 + -(-K // 128) + 16) * 2.0 ** -24 + (2.0 ** -12 if dtype != "f32" and rows > 64 else 0)
+    limit = size * (1.13 * off + 2.0 ** -21) + ref.half_step(dtype) * np.abs(want) * (1 + 2.0 ** -8) + ref.smallest_step(dtype)
+    assert np.all(np.abs(got - want) <= limit), (np.abs(got - want) / limit).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K,N", [
+    (1, 1, 1), (1, 128, 16), (1, 4096, 200), (3, 127, 33), (16, 2048, 130), (17, 129, 129), (31, 640, 500), (33, 384, 257),
+    (64, 272, 1000), (65, 128, 128), (70, 16, 300), (129, 777, 131), (200, 400, 1001), (256, 1024, 512), (300, 2100, 77), (513, 145, 640)])
+def test_matmul_blocks(om, M, K, N, dtype):
+    rng = np.random.default_rng(M + K + N)
+    a, sa, b, sb = operands(om, rng, M, K, N)
+    got = om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), on(om, sb), dtype=dt(om, dtype))
+    want, size = product(om, a, sa, b, sb)
+    check_product(om, back(om, got), want, size, dtype, M, K)
+
+
+@pytest.mark.parametrize("act", [0, 1, 2])
+@pytest.mark.parametrize("M", [2, 90])
+@pytest.mark.parametrize("bias", ["none", "one", "columns"])
+def test_matmul_blocks_bias_and_activation(om, M, bias, act):
+    rng = np.random.default_rng(M + act)
+    K, N = 300, 150
+    a, sa, b, sb = operands(om, rng, M, K, N)
+    c = {"none": None, "one": np.float32([0.3]), "columns": rng.standard_normal(N).astype(np.float32)}[bias]
+    got = om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), on(om, sb), None if c is None else on(om, c), act)
+    want, size = product(om, a, sa, b, sb, c, act)
+    check_product(om, back(om, got), want, size, "f32", M, K)
+
+
+@pytest.mark.parametrize("M", [2, 90])
+def test_matmul_blocks_without_elements_of_k(om, M):
+    c = np.arange(5, dtype=np.float32)
+    got = om.MatMulBlocks(np.zeros((M, 0), om.float8_e4m3fn), np.zeros((M, 0), np.float32), np.zeros((5, 0), om.float8_e4m3fn),
+                          np.zeros((1, 0), np.float32), c)
+    assert np.array_equal(got, np.tile(c, (M, 1)))
+
+
+@pytest.mark.parametrize("M", [5, 100])
+@pytest.mark.parametrize("shift", [1, 8])
+def test_matmul_blocks_at_any_address(om, M, shift):
+    rng = np.random.default_rng(M)
+    K, N = 256, 48
+    a, sa, b, sb = operands(om, rng, M, K, N)
+
+    def moved(x):
+        flat = np.zeros(x.size + shift, x.dtype)
+        flat[shift:] = x.reshape(-1)
+        return om.DeviceArray.view_of(on(om, flat), shift, x.shape)
+
+    got = om.MatMulBlocks(moved(a), on(om, sa), moved(b), on(om, sb))
+    want, size = product(om, a, sa, b, sb)
+    check_product(om, back(om, got), want, size, "f32", M, K)
+
+
+@pytest.mark.parametrize("M", [3, 80])
+def test_matmul_blocks_nan_stays_in_its_row_and_column(om, M):
+    """Codes behind the last element of a row (here the next row's) are not read as
+    part of it, NaN among them."""
+    rng = np.random.default_rng(M)
+    K, N = 144, 40
+    a, sa, b, sb = operands(om, rng, M, K, N)
+    a["bits"][1, 0] = 0x7F
+    b["bits"][7, 0] = 0xFF
+    want, size = product(om, a, sa, b, sb)
+    got = back(om, om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), on(om, sb)))
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want[1]).all() and np.isnan(want[:, 7]).all()
+    ok = ~np.isnan(want)
+    check_product(om, got[ok], want[ok], size[ok], "f32", M, K)
+
+
+def test_matmul_blocks_leading_dimensions_and_host_arrays(om):
+    rng = np.random.default_rng(3)
+    a, sa, b, sb = operands(om, rng, 6, 200, 50)
+    got = om.MatMulBlocks(a.reshape(2, 3, 200), sa.reshape(2, 3, 2), b, sb, dtype=om.bfloat16)
+    want, size = product(om, a, sa, b, sb)
+    assert got.shape == (2, 3, 50) and got.dtype == om.bfloat16
+    check_product(om, back(om, got).reshape(6, 50), want, size, "bf16", 6, 200)
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+def pack_heads(x, heads_first):
+    """[B, H, S, D] as it is, or as [B, S, H * D]."""
+    return np.ascontiguousarray(x) if heads_first else np.ascontiguousarray(np.swapaxes(x, 1, 2).reshape(x.shape[0], x.shape[2], -1))
+
+
+def unpack_heads(y, heads, heads_first):
+    return y if heads_first else np.swapaxes(y.reshape(y.shape[0], y.shape[1], heads, -1), 1, 2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("B,H,S,D,rot,heads_first,ids", [
+    (1, 1, 1, 2, 2, True, True), (2, 3, 5, 64, 64, True, True), (2, 3, 5, 64, 64, False, True), (3, 2, 7, 80, 80, False, False),
+    (1, 4, 9, 128, 64, True, True), (2, 2, 3, 96, 10, False, True), (1, 3, 2, 13, 6, True, False), (2, 1, 33, 256, 128, False, True),
+    (1, 2, 4, 32, 0, True, True)])
+def test_rotary(om, B, H, S, D, rot, heads_first, ids, interleaved, dtype):
+    rng = np.random.default_rng(B + H + S + D)
+    x = om.from_float32(rng.standard_normal((B, H, S, D)), dt(om, dtype))
+    half = (rot or D) // 2
+    cos, sin = om.rotary_tables(50, 2 * half, scaling="linear", factor=2.0)
+    pos = rng.integers(0, 50, (B, S)).astype(np.int64)
+    c, s = cos[pos], sin[pos]
+    given = (cos, sin, on(om, pos)) if ids else (c, s, None)
+    d = on(om, pack_heads(x, heads_first))
+    got = om.RotaryEmbedding(d, on(om, given[0]), on(om, given[1]), given[2], interleaved, 0 if heads_first else H, rot)
+    v = om.to_float32(x)
+    want = ref.rotate(v, c, s, 2 * half, interleaved)
+    # two products and their sum in f32, then the type's rounding
+    size = np.abs(v).max() * 2
+    limit = 3 * 2.0 ** -24 * size + ref.half_step(dtype) * np.abs(want) * (1 + 2.0 ** -20) + ref.smallest_step(dtype)
+    out = unpack_heads(back(om, got), H, heads_first)
+    assert np.all(np.abs(out - want) <= limit)
+    assert np.array_equal(out[..., 2 * half:], v[..., 2 * half:])
+    # in place
+    om.RotaryEmbedding(d, on(om, given[0]), on(om, given[1]), given[2], interleaved, 0 if heads_first else H, rot, out=d)
+    assert np.array_equal(back(om, d), back(om, got))
+
+
+def test_rotary_positions_that_the_tables_do_not_hold(om):
+    x = np.ones((1, 2, 4, 64), np.float32)
+    cos, sin = om.rotary_tables(3, 32)
+    got = back(om, om.RotaryEmbedding(on(om, x), on(om, cos), on(om, sin), on(om, np.array([[0, 3, -1, 2 ** 40]], np.int64)),
+                                      rotary_embedding_dim=32))
+    assert np.isfinite(got[0, :, 0]).all() and np.isnan(got[0, :, 1:, :32]).all() and (got[..., 32:] == 1).all()
+
+
+# ---------------------------------------------------------------------------
+# the cache
+# ---------------------------------------------------------------------------
+def random_cache(om, rng, pages, H, size, D):
+    """A cache with something in every place."""
+    c = om.Cache4(pages, H, size, D)
+    c.k_codes, c.k_scales = ref.quantize4(rng.standard_normal((pages, H, size, D)).astype(np.float32))
+    c.v_codes, c.v_scales = ref.quantize4(rng.standard_normal((pages, H, size, D)).astype(np.float32))
+    return c
+
+
+def to_gpu(om, c):
+    d = om.Cache4(1, 1, 16, 64)
+    d.k_codes, d.k_scales, d.v_codes, d.v_scales = [on(om, np.ascontiguousarray(t)) for t in c.tensors]
+    return d
+
+
+def tables_of(rng, B, each, extra=1):
+    return rng.permutation(B * each + extra)[:B * each].reshape(B, each).astype(np.int32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,H,S,D,size,paged,heads_first,ragged", [
+    (1, 1, 1, 64, 16, True, True, False), (3, 2, 5, 96, 16, True, False, True), (2, 3, 40, 128, 48, True, True, True),
+    (2, 1, 17, 192, 64, False, False, False), (4, 2, 3, 256, 21, False, True, True), (2, 4, 33, 128, 32, True, False, False)])
+def test_append(om, B, H, S, D, size, paged, heads_first, ragged, dtype):
+    rng = np.random.default_rng(B * H * S + D)
+    each = (S + 20) // size + 1 if paged else 1
+    if not paged:
+        size = max(size, S + 2)
+    table = tables_of(rng, B, each) if paged else None
+    pages = B * each + 1
+    c = random_cache(om, rng, pages, H, size, D)
+    past = rng.integers(0, each * size - S + 1, B).astype(np.int32)
+    counts = rng.integers(0, S + 1, B).astype(np.int32) if ragged else None
+    k, v = (om.from_float32(awkward(rng, (B, H, S, D)), dt(om, dtype)) for _ in range(2))
+    k["bits" if dtype == "bf16" else ...][0, 0, 0] = 0  # a row of zeros
+    want = [t.copy() for t in c.tensors]
+    for x, codes, scales in ((k, want[0], want[1]), (v, want[2], want[3])):
+        qc, qs = ref.quantize4(om.to_float32(x))
+        for b in range(B):
+            for i in range(S if counts is None else counts[b]):
+                t = past[b] + i
+                page = table[b, t // size] if paged else b
+                codes[page, :, t % size], scales[page, :, t % size] = qc[b, :, i], qs[b, :, i]
+    d = to_gpu(om, c)
+    om.CacheAppend4(d, on(om, pack_heads(k, heads_first)), on(om, pack_heads(v, heads_first)), on(om, past),
+                    None if table is None else on(om, table), None if counts is None else on(om, counts))
+    for g, w in zip(d.tensors, want):
+        assert np.array_equal(g.numpy(), w)
+    # host arrays, checked and copied both ways
+    om.CacheAppend4(c, pack_heads(k, heads_first), pack_heads(v, heads_first), past, table, counts)
+    for g, w in zip(c.tensors, want):
+        assert np.array_equal(g, w)
+
+
+def test_append_extreme_values(om):
+    """Infinities and what f16 cannot hold are limited, NaN marks its group, a
+    group of tiny values gets the scale 0."""
+    x = np.zeros((1, 1, 1, 256), np.float32)
+    r = x[0, 0, 0].reshape(8, 32)
+    r[0, :3] = np.inf, -np.inf, 1.0
+    r[1, :2] = 1e30, -7.0
+    r[2, 5] = np.nan
+    r[3] = 3.14159
+    r[4] = 1e-9
+    r[5] = np.linspace(-65000, 65504, 32)
+    r[6] = 2.0 ** -24 * np.arange(32)
+    r[7] = np.linspace(0, 15, 32)
+    c = om.Cache4(1, 1, 16, 256, template=on(om, x))
+    om.CacheAppend4(c, on(om, x), on(om, x), on(om, np.zeros(1, np.int32)))
+    codes, scales = ref.quantize4(x)
+    for g, w in zip(c.tensors, (codes, scales) * 2):
+        assert equal(g.numpy()[0, :, :1].astype(np.float32), w[0].astype(np.float32))
+    s = scales[0, 0, 0].astype(np.float64)
+    # (3.14159 in f16 is 3.140625: the group has a scale for what is left)
+    assert np.isnan(s[2]).all() and s[3, 1] == 3.140625 and s[3, 0] > 0 and s[4, 0] == 0 and s[0, 1] == -65504 and np.isfinite(np.delete(s, 2, 0)).all()
+
+
+def test_tokens_without_a_place_are_not_stored(om):
+    """Tables and lengths in GPU memory: pages that are none, tokens past the pages."""
+    rng = np.random.default_rng(1)
+    c = random_cache(om, rng, 3, 2, 16, 64)
+    d = to_gpu(om, c)
+    k = rng.standard_normal((3, 2, 20, 64)).astype(np.float32)
+    table = np.array([[0, 7], [-1, 1], [2, -5]], np.int32)
+    om.CacheAppend4(d, on(om, k), on(om, k), on(om, np.array([0, 13, -2], np.int32)), on(om, table), on(om, np.array([20, 99, -4], np.int32)))
+    want = [t.copy() for t in c.tensors]
+    qc, qs = ref.quantize4(k)
+    for codes, scales in ((want[0], want[1]), (want[2], want[3])):
+        codes[0], scales[0] = qc[0][:, :16], qs[0][:, :16]          # page 7 is none
+        codes[1], scales[1] = qc[1][:, 3:19], qs[1][:, 3:19]        # its first page is none, and token 32 has none
+    for g, w in zip(d.tensors, want):
+        assert np.array_equal(g.numpy(), w)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def check_attention(om, got, want, sure, dtype):
+    """Scores: f32 sums of 32 G exact products, G scalings and sums, lowest values:
+    2^-24 of sum |q khat| for each of at most 300 roundings, then the exponential's
+    2^-22.  Weights are off by twice that, relatively; sums over n keys by
+    (n + 64) 2^-24; weights times scales are held to 2^-16 (16-bit results) or
+    2^-23."""
+    score = 300 * 2.0 ** -24 * (1 + sure[..., 0]) + 2.0 ** -22
+    split = 2.0 ** -23 if dtype == "f32" else 2.0 ** -16
+    off = 2 * score * sure[..., 1] + ((sure[..., 3] + 64) * 2.0 ** -24 + split) * sure[..., 2]
+    seen = ~np.isnan(want)
+    limit = off[..., None] + ref.half_step(dtype) * np.abs(want) * (1 + 2.0 ** -7) + ref.smallest_step(dtype)
+    assert np.all(np.abs(got - want)[seen] <= limit[seen]), (np.abs(got - want) / limit)[seen].max()
+
+
+CASES = [
+    # B, Hq, H, S, D, page size, paged, past, options
+    (1, 1, 1, 1, 64, 16, True, [0], {}),
+    (1, 4, 1, 1, 128, 16, True, [31], {}),
+    (2, 8, 2, 1, 128, 48, True, [15, 300], {}),
+    (3, 7, 7, 1, 64, 16, True, [0, 16, 33], {}),
+    (2, 12, 4, 1, 96, 64, True, [100, 63], {}),
+    (1, 8, 1, 1, 256, 130, False, [128], {}),
+    (2, 6, 2, 1, 192, 77, False, [76, 3], {}),
+    (1, 2, 2, 17, 64, 16, True, [5], {}),
+    (2, 8, 2, 9, 128, 16, True, [40, 0], {}),
+    (1, 3, 1, 40, 96, 100, False, [20], {}),
+    (2, 4, 2, 33, 128, 64, True, [64, 1], {"causal": 0}),
+    (2, 4, 2, 20, 128, 16, True, [64, 30], {"window": 7}),
+    (1, 4, 4, 1, 64, 16, True, [500], {"window": 33}),
+    (3, 4, 1, 1, 128, 16, True, [50, 50, 50], {"starts": [0, 20, 51]}),
+    (2, 2, 1, 12, 64, 32, True, [10, 10], {"starts": [5, 15], "window": 6}),
+    (2, 2, 1, 12, 64, 32, True, [10, 10], {"starts": [30, 3], "causal": 0}),
+    (3, 4, 2, 10, 128, 16, True, [0, 33, 7], {"counts": [10, 0, 3]}),
+    (2, 4, 2, 10, 96, 16, True, [0, 33], {"counts": [0, 4], "causal": 0}),
+    (1, 4, 1, 2, 128, 16, True, [3], {"scale": 0.0}),
+    (1, 4, 1, 2, 128, 16, True, [70], {"scale": -1.5}),
+    (1, 16, 2, 1, 128, 16, True, [2000], {}),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads_first", [True, False])
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention(om, case, heads_first, dtype):
+    B, Hq, H, S, D, size, paged, past, options = CASES[case]
+    options = dict(options)
+    rng = np.random.default_rng(case)
+    each = max(p + S - 1 for p in past) // size + 2 if paged else 1
+    table = tables_of(rng, B, each) if paged else None
+    c = random_cache(om, rng, B * each + 1, H, size, D)
+    counts = options.get("counts")
+    # places that no token of a sequence takes hold NaN, as do their pages' numbers nothing
+    for b in range(B):
+        n = past[b] + (S if counts is None else counts[b])
+        for t in range(n, each * size):
+            page = table[b, t // size] if paged else b
+            c.k_scales[page, :, t % size] = np.nan
+            c.v_scales[page, :, t % size] = np.inf
+        if paged:
+            table[b, -(-n // size):] = [-1, 10 ** 6][b % 2]
+    q = om.from_float32(rng.standard_normal((B, Hq, S, D)), dt(om, dtype))
+    arrays = {k: np.array(v, np.int32) for k, v in options.items() if k in ("counts", "starts")}
+    scale = np.float32(options["scale"]) if "scale" in options else None
+    want, sure = ref.attention(om.to_float32(q), c.tensors, past, None if table is None else np.clip(table, 0, B * each),
+                               arrays.get("counts"), arrays.get("starts"), scale, options.get("causal", 1), options.get("window", 0))
+    before = om.from_float32(np.full(q.shape, 77.0), dt(om, dtype))
+    kinds = dict(causal=options.get("causal", 1), window=options.get("window", 0))
+    out = on(om, pack_heads(before, heads_first))
+    om.CacheAttention4(on(om, pack_heads(q, heads_first)), to_gpu(om, c), on(om, np.array(past, np.int32)),
+                       None if table is None else on(om, table), scale=None if scale is None else on(om, scale), out=out,
+                       **{k: on(om, v) for k, v in arrays.items()}, **kinds)
+    got = unpack_heads(back(om, out), Hq, heads_first)
+    assert np.array_equal(got[np.isnan(want)], np.full(np.isnan(want).sum(), 77.0, np.float32))  # rows behind the last token
+    assert np.isfinite(got).all()
+    check_attention(om, got, want, sure, dtype)
+    if heads_first:  # host arrays give the same bits
+        again = before.copy()
+        om.CacheAttention4(q, c, np.array(past, np.int32), table, scale=scale, out=again, **arrays, **kinds)
+        assert np.array_equal(om.to_float32(again), got)
+
+
+def test_attention_nan_of_one_sequence_stays_there(om):
+    """NaN in a key that a row sees reaches that row, and not the row before it."""
+    rng = np.random.default_rng(0)
+    c = random_cache(om, rng, 2, 1, 64, 64)
+    c.k_scales[0, 0, 10, 1] = np.nan
+    c.v_scales[0, 0, 12, 0] = np.inf
+    q = rng.standard_normal((2, 1, 20, 64)).astype(np.float32)
+    got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.zeros(2, np.int32))))
+    assert np.isfinite(got[0, 0, :10]).all() and np.isnan(got[0, 0, 10:]).all() and np.isfinite(got[1]).all()
+
+
+def test_attention_of_sharp_and_flat_scores(om):
+    """Scores hundreds apart in both orders: what is kept relative to an old maximum
+    does not overflow, and what is far below a new one vanishes."""
+    rng = np.random.default_rng(2)
+    D, n = 128, 300
+    k = rng.standard_normal((1, 1, n, D)).astype(np.float32)
+    k *= np.linspace(0.01, 20, n, dtype=np.float32)[None, None, :, None]
+    v = rng.standard_normal((1, 1, n, D)).astype(np.float32)
+    q = np.concatenate([k[:, :, -1:] * 0.3, k[:, :, :1] * 100, -k[:, :, -1:]], 1).astype(np.float32)  # 3 heads
+    for order in (1, -1):
+        c = om.Cache4(1, 1, n, D)
+        c.k_codes, c.k_scales = ref.quantize4(k[:, :, ::order])
+        c.v_codes, c.v_scales = ref.quantize4(v)
+        got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.array([n - 1], np.int32))))
+        want, sure = ref.attention(q, c.tensors, [n - 1])
+        check_attention(om, got, want, sure, "f32")
+
+
+def test_a_decoder_layers_attention_block(om):
+    """The ops as a decoder uses them, two prompts of different lengths and then two
+    more tokens of each: every step against what its own inputs say."""
+    rng = np.random.default_rng(9)
+    B, H, KV, D, hidden = 2, 4, 2, 64, 256
+    wide = (H + 2 * KV) * D
+    w, ws = om.DynamicQuantizeBlocks(on(om, (0.05 * rng.standard_normal((wide, hidden))).astype(np.float32)), 128)
+    wo, wos = om.DynamicQuantizeBlocks(on(om, (0.05 * rng.standard_normal((hidden, H * D))).astype(np.float32)), 128)
+    cos, sin = (on(om, t) for t in om.rotary_tables(64, D))
+    cache = to_gpu(om, random_cache(om, rng, 7, KV, 16, D))
+    table = np.array([[3, 0, 5], [1, 6, 2]], np.int32)
+    past, lengths = np.zeros(2, np.int32), np.array([19, 30], np.int32)
+    held = {b: ([], []) for b in range(B)}
+    for S, counts in ((30, lengths), (1, None), (1, None)):
+        x = om.from_float32(rng.standard_normal((B, S, hidden)), om.bfloat16)
+        xq, xs = om.DynamicQuantizeBlocks(on(om, x))
+        qkv = om.MatMulBlocks(xq, xs, w, ws, dtype=om.bfloat16)
+        host = qkv.numpy()
+        want, size = product(om, xq.numpy().reshape(-1, hidden), xs.numpy().reshape(B * S, -1), w.numpy(), ws.numpy())
+        check_product(om, om.to_float32(host).reshape(B * S, wide), want, size, "bf16", B * S, hidden)
+        q, k, v = (np.ascontiguousarray(host[..., a * D:b * D]) for a, b in ((0, H), (H, H + KV), (H + KV, H + 2 * KV)))
+        pos = on(om, past[:, None].astype(np.int64) + np.arange(S))
+        q = om.RotaryEmbedding(on(om, q), cos, sin, pos, num_heads=H)
+        k = om.RotaryEmbedding(on(om, k), cos, sin, pos, num_heads=KV)
+        n = None if counts is None else on(om, counts)
+        om.CacheAppend4(cache, k, on(om, v), on(om, past), on(om, table), n)
+        y = om.CacheAttention4(q, cache, on(om, past), on(om, table), n, out=on(om, np.zeros((B, S, H * D), om.bfloat16)))
+        full = [t.numpy() for t in cache.tensors]
+        want, sure = ref.attention(unpack_heads(back(om, q), H, False), full, past, table, counts)
+        check_attention(om, unpack_heads(back(om, y), H, False), np.where(np.isnan(want), 0, want), sure, "bf16")
+        # the cache holds what was appended
+        kr, vr = unpack_heads(back(om, k), KV, False), unpack_heads(om.to_float32(v), KV, False)
+        for b in range(B):
+            m = S if counts is None else counts[b]
+            held[b][0].append(kr[b, :, :m])
+            held[b][1].append(vr[b, :, :m])
+            for one, codes, scales in zip(held[b], full[::2], full[1::2]):
+                rows = np.concatenate(one, 1)
+                c, s = ref.quantize4(rows)
+                assert np.array_equal(ref.rows_of(codes, table, b)[:, :rows.shape[1]], c)
+                assert np.array_equal(ref.rows_of(scales, table, b)[:, :rows.shape[1]], s)
+        yq, ys = om.DynamicQuantizeBlocks(y)
+        o = om.MatMulBlocks(yq, ys, wo, wos)
+        want, size = product(om, yq.numpy().reshape(-1, H * D), ys.numpy().reshape(B * S, -1), wo.numpy(), wos.numpy())
+        check_product(om, back(om, o).reshape(B * S, hidden), want, size, "f32", B * S, H * D)
+        past = (past + (S if counts is None else counts)).astype(np.int32)
+
+
+def test_two_threads_at_once(om):
+    """Each thread has a stream and workspaces of its own."""
+    import threading
+    rng = np.random.default_rng(4)
+    c = to_gpu(om, random_cache(om, rng, 2, 2, 512, 128))
+    q = rng.standard_normal((2, 8, 1, 128)).astype(np.float32)
+    past = on(om, np.array([500, 300], np.int32))
+    dq = on(om, q)
+    want = om.CacheAttention4(dq, c, past).numpy()
+    a, sa, b, sb = operands(om, rng, 70, 300, 100)
+    args = [on(om, t) for t in (a, sa, b, sb)]
+    wy = om.MatMulBlocks(*args).numpy()
+    wrong = []
+
+    def work():
+        for _ in range(20):
+            if not np.array_equal(om.CacheAttention4(dq, c, past).numpy(), want) or not np.array_equal(om.MatMulBlocks(*args).numpy(), wy):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
