@@ -9,6 +9,8 @@
 // 8 elements of every group, and G neighbouring bytes of a value's row are the
 // elements (2 n, 2 n + 1) of every group.
 
+#include <type_traits>
+
 #include "llm_common.h"
 
 namespace om {
@@ -126,13 +128,21 @@ __global__ __launch_bounds__(256) void k_cache_append(const Append4 p) {
 // for bf16, f16, f32), and 2 (16-bit results) or 3 for p s.  Sums, scores and
 // softmax statistics are f32.
 //
-// A wave takes 16 RT rows (queries of the heads that share one of keys) and 32
-// keys at a time.  Keys are the first operand of the first product and elements
-// of a value that of the second, so that lane (c, h) holds row c throughout:
-// scores of keys 4 h .. of either 16, which are also its places of the second
-// product's operand, and output elements 32 g + 8 h ...  Nothing is moved
-// between lanes but the rows' maxima, and those only when one grows by more
-// than 8 (powers of two) over what p is relative to.
+// A wave takes RT tiles of rows (queries of the heads that share one of keys)
+// and 32 keys at a time.  Keys are the first operand of the first product and
+// elements of a value that of the second, so that lane (c, h) holds column c of
+// either throughout: scores of keys 4 h .. of each 16, which are also its places
+// of the second product's operand.  No score moves between lanes but the rows'
+// maxima, and those only when one grows by more than 8 (powers of two) over
+// what p is relative to.
+//
+// A tile's 16 columns are 16 rows; or, where there are few, PACKED: 16 / G rows
+// times G groups.  Column (g, r) of q then holds group g of row r and zeros, its
+// products that group's part of the score, to be scaled by the one scale the
+// lane has and summed over the columns of the row; and its weights are scaled
+// for group g, of whose elements alone the results are kept.  The matrix
+// instructions are as many, the vector ones, which bound the kernel, less than
+// half: a lane scales and splits 8 weights for 32 keys, not 8 G.
 struct Arguments {
   Cache4 c;
   const void *q;
@@ -146,34 +156,25 @@ struct Arguments {
   bool causal, heads_first;
 };
 
-// Bytes a.g and b.g of words a and b, then those of g + 1.
-__device__ __forceinline__ unsigned two_of(unsigned a, unsigned b, int byte) {
-  const unsigned s = (unsigned)byte;
-  return __builtin_amdgcn_perm(b, a, s | (4 + s) << 8 | (s + 1) << 16 | (5 + s) << 24);
-}
-__device__ __forceinline__ unsigned one_of(
-    unsigned a, int ia, unsigned b, int ib) {
-  return __builtin_amdgcn_perm(b, a, (unsigned)ia | (unsigned)(4 + ib) << 8);
-}
-
-// Byte at[i] + g of word string i, for i = 0 .. 3 and every g: codes[g].
+// Bytes at[i] + g of the four strings w[i], for i = 0 .. 3 and every g.
 template <int G, int STEP, int WORDS>
 __device__ __forceinline__ void bytes_of(
-    const unsigned (&w)[4][WORDS], unsigned (&codes)[G]) {
+    const unsigned *const (&w)[4], unsigned (&codes)[G]) {
 #pragma unroll
   for (int g = 0; g < G; g += G % 2 ? 1 : 2) {
-    auto word = [&](int i) { return w[i][(i * STEP + g) / 4]; };
-    auto byte = [&](int i) { return (i * STEP + g) % 4; };
+    const unsigned w0 = w[0][g / 4], w1 = w[1][(STEP + g) / 4],
+                   w2 = w[2][(2 * STEP + g) / 4], w3 = w[3][(3 * STEP + g) / 4];
+    const unsigned s0 = g % 4, s1 = (STEP + g) % 4, s2 = (2 * STEP + g) % 4,
+                   s3 = (3 * STEP + g) % 4;
     if (G % 2) {
-      const unsigned x = one_of(word(0), byte(0), word(1), byte(1));
-      const unsigned y = one_of(word(2), byte(2), word(3), byte(3));
+      const unsigned x = __builtin_amdgcn_perm(w1, w0, s0 | (4 + s1) << 8);
+      const unsigned y = __builtin_amdgcn_perm(w3, w2, s2 | (4 + s3) << 8);
       codes[g] = __builtin_amdgcn_perm(y, x, 0x05040100);
     } else {
-      const unsigned s0 = byte(0), s1 = byte(1), s2 = byte(2), s3 = byte(3);
       const unsigned x = __builtin_amdgcn_perm(
-          word(1), word(0), s0 | (4 + s1) << 8 | (s0 + 1) << 16 | (5 + s1) << 24);
+          w1, w0, s0 | (4 + s1) << 8 | (s0 + 1) << 16 | (5 + s1) << 24);
       const unsigned y = __builtin_amdgcn_perm(
-          word(3), word(2), s2 | (4 + s3) << 8 | (s2 + 1) << 16 | (5 + s3) << 24);
+          w3, w2, s2 | (4 + s3) << 8 | (s2 + 1) << 16 | (5 + s3) << 24);
       codes[g] = __builtin_amdgcn_perm(y, x, 0x05040100);
       codes[g + 1] = __builtin_amdgcn_perm(y, x, 0x07060302);
     }
@@ -193,34 +194,82 @@ __device__ __forceinline__ v8bf join(v2bf a, v2bf b, v2bf c, v2bf d) {
 // x as a sum of N bf16 values, each the nearest to what the ones before leave.
 template <int N>
 __device__ __forceinline__ void terms_of(const float (&x)[8], v8bf (&t)[N]) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  v2bf part[N][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float rest = x[i];
+  for (int i = 0; i < 4; ++i) {
+    float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      t[k][i] = (__bf16)rest;
-      if (k + 1 < N)
-        rest -= to_f32(t[k][i]);
+      part[k][i] = __builtin_convertvector(v2f{a, b}, v2bf);
+      if (k + 1 < N) {
+        const unsigned w = __builtin_bit_cast(unsigned, part[k][i]);
+        a -= __builtin_bit_cast(float, w << 16);
+        b -= __builtin_bit_cast(float, w & 0xFFFF0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    t[k] = join(part[k][0], part[k][1], part[k][2], part[k][3]);
+}
+
+// N words (or, with B, bytes) at a lane's offset from what a descriptor covers;
+// behind its end lie zeros.
+template <int N>
+__device__ __forceinline__ void load_words(
+    __amdgpu_buffer_rsrc_t from, int at, unsigned (&w)[N]) {
+  constexpr int W = N % 4 == 0 ? 4 : N % 3 == 0 ? 3 : N;
+  static_assert(W <= 4, "words of a load");
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    if constexpr (W == 4) {
+      const v4u v = __builtin_amdgcn_raw_buffer_load_b128(from, at + 4 * i, 0, 0);
+      w[i] = v[0], w[i + 1] = v[1], w[i + 2] = v[2], w[i + 3] = v[3];
+    } else if constexpr (W == 3) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b96(from, at + 4 * i, 0, 0);
+      w[i] = v[0], w[i + 1] = v[1], w[i + 2] = v[2];
+    } else if constexpr (W == 2) {
+      const v2u v = __builtin_amdgcn_raw_buffer_load_b64(from, at + 4 * i, 0, 0);
+      w[i] = v[0], w[i + 1] = v[1];
+    } else {
+      w[i] = __builtin_amdgcn_raw_buffer_load_b32(from, at + 4 * i, 0, 0);
     }
   }
 }
-
-// N bytes from an address aligned to `ALIGN`.
-template <int N, int ALIGN>
+template <int B>
 __device__ __forceinline__ void load_bytes(
-    const uint8_t *p, unsigned (&w)[(N + 3) / 4]) {
-  struct alignas(ALIGN) Bytes {
-    uint8_t b[N];
-  };
-  const Bytes v = *(const Bytes *)p;
+    __amdgpu_buffer_rsrc_t from, int at, unsigned (&w)[(B + 3) / 4]) {
+  if constexpr (B % 4 == 0) {
+    load_words<B / 4>(from, at, w);
+  } else {
+    constexpr int P = B % 2 ? 1 : 2; // bytes of a load
 #pragma unroll
-  for (int i = 0; i < (N + 3) / 4; ++i) {
-    w[i] = 0;
+    for (int i = 0; i < (B + 3) / 4; ++i)
+      w[i] = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * i + j < N)
-        w[i] |= (unsigned)v.b[4 * i + j] << (8 * j);
+    for (int i = 0; i < B; i += P)
+      w[i / 4] |= (unsigned)(P == 2 ? (unsigned)__builtin_amdgcn_raw_buffer_load_b16(from, at + i, 0, 0)
+                                    : (unsigned)__builtin_amdgcn_raw_buffer_load_b8(from, at + i, 0, 0))
+                  << (8 * (i % 4));
   }
+}
+
+// The sum over the G columns of a row (lanes c, c + 16 / G, ..), in all of them:
+// each step adds what the other half of a rotation holds, so every lane adds the
+// same numbers in the same order.
+template <int G> __device__ __forceinline__ float columns_sum(float v) {
+#define OM_ROW_ADD(ctrl)                                                       \
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(                    \
+                                     0, __builtin_bit_cast(int, v), ctrl, 0xF,   \
+                                     0xF, true))
+  OM_ROW_ADD(0x128); // row_ror:8
+  if (G > 2)
+    OM_ROW_ADD(0x124);
+  if (G > 4)
+    OM_ROW_ADD(0x122);
+#undef OM_ROW_ADD
+  return v;
 }
 
 constexpr int kWaves = 4;
@@ -231,21 +280,25 @@ template <> struct Terms<float> { static constexpr int q = 3, p = 3; };
 template <> struct Terms<_Float16> { static constexpr int q = 2, p = 2; };
 template <> struct Terms<__bf16> { static constexpr int q = 1, p = 2; };
 
-template <typename T, int G, int RT>
-__global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments p) {
+template <typename T, int G, int RT, bool PACKED>
+__global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_cache_attention(const Arguments p) {
   constexpr int D = 32 * G, TQ = Terms<T>::q, TP = Terms<T>::p;
+  constexpr int ROWS = PACKED ? 16 / G : 16; // of a tile
+  constexpr int SG = PACKED ? 1 : G;         // groups whose scales a lane holds
+  static_assert(!PACKED || 16 % G == 0, "columns");
   extern __shared__ __attribute__((aligned(16))) float shared[];
   const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int my_row = PACKED ? c % ROWS : c, my_group = PACKED ? c / ROWS : 0;
   const float inf = __builtin_inff();
 
   // Blocks of one head of keys are neighbours: an XCD's L2 holds it once.
-  int id = xcd_contiguous(blockIdx.x, (int)gridDim.x);
-  const int split = id % p.splits;
-  const int unit = id / p.splits;
-  const int group = unit % p.groups;
-  const int bh = unit / p.groups;
-  const int b = bh / p.c.H, head = bh % p.c.H;
+  const int id = xcd_contiguous(blockIdx.x, (int)gridDim.x);
+  const int split = (unsigned)id % (unsigned)p.splits;
+  const int unit = (unsigned)id / (unsigned)p.splits;
+  const int group = (unsigned)unit % (unsigned)p.groups;
+  const int bh = (unsigned)unit / (unsigned)p.groups;
+  const int b = (unsigned)bh / (unsigned)p.c.H, head = (unsigned)bh % (unsigned)p.c.H;
 
   const int past = p.c.past[b];
   int count = p.S;
@@ -253,14 +306,14 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
     const int n = p.c.counts[b];
     count = n < 0 ? 0 : n < p.S ? n : p.S;
   }
-  const int rows = count * p.per_head, row0 = group * RT * 16;
+  const int rows = count * p.per_head, row0 = group * RT * ROWS;
   if (row0 >= rows)
     return;
-  const int last_row = (row0 + RT * 16 < rows ? row0 + RT * 16 : rows) - 1;
-  const int64_t capacity =
-      p.c.table ? p.c.table_pages * p.c.page_size : p.c.page_size;
+  const int last_row = (row0 + RT * ROWS < rows ? row0 + RT * ROWS : rows) - 1;
+  const unsigned page_size = (unsigned)p.c.page_size;
+  const int capacity = (int)(p.c.table ? p.c.table_pages * p.c.page_size : p.c.page_size);
   // Keys [first, end) of the query of token i.
-  const int64_t start = p.starts ? p.starts[b] : 0;
+  const int start = p.starts ? p.starts[b] : 0;
   auto first_of = [&](int i) -> int {
     int64_t f = start > 0 ? start : 0;
     if (p.window > 0 && past + (int64_t)i - p.window + 1 > f)
@@ -274,20 +327,23 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
   const int i0 = row0 / p.per_head, i1 = last_row / p.per_head;
   const int lo = first_of(i0), hi = end_of(i1);
   const int all_lo = first_of(i1), all_hi = end_of(i0); // seen by all rows
+  // Tiles of 32 keys: this part's, of which the wave takes every kWaves-th.
   int tile = lo / 32, tiles = hi > lo ? (hi + 31) / 32 - tile : 0;
   {
     const int each = (tiles + p.splits - 1) / p.splits;
     tile += split * each;
     tiles = tiles - split * each < each ? tiles - split * each : each;
+    tile += wave;
+    tiles = tiles > wave ? (tiles - wave + kWaves - 1) / kWaves : 0;
   }
 
   // This lane's rows.
   v8bf q[RT][G][TQ];
-  float qsum[RT][G];
+  float qsum[RT][SG];
   int row_lo[RT], row_hi[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    int row = row0 + 16 * r + c;
+    int row = row0 + ROWS * r + my_row;
     row = row < rows ? row : rows - 1;
     const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
     row_lo[r] = first_of(i);
@@ -295,15 +351,22 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
     const int64_t at = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
                                      : ((int64_t)b * p.S + i) * p.heads + qh;
     const T *const x = (const T *)p.q + at * D + 8 * h;
+    if (PACKED)
+      qsum[r][0] = 0.0f;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
+      const bool held = !PACKED || g == my_group;
       float v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        v[j] = to_f32(x[32 * g + j]);
+        v[j] = held ? to_f32(x[32 * g + j]) : 0.0f;
       float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       sum += __shfl_xor(sum, 16);
-      qsum[r][g] = sum + __shfl_xor(sum, 32);
+      sum += __shfl_xor(sum, 32);
+      if (PACKED)
+        qsum[r][0] = held ? sum : qsum[r][0];
+      else
+        qsum[r][g] = sum;
       const float order[8] = {v[0], v[2], v[4], v[6], v[1], v[3], v[5], v[7]};
       terms_of<TQ>(order, q[r][g]);
     }
@@ -312,70 +375,96 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
       (p.scale ? p.scale[0] : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
 
   v4f o[RT][2 * G];
-  float top[RT], sum[RT], low[RT][G]; // low: sum of p m
+  float top[RT], sum[RT], low[RT][SG]; // low: sum of p m
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     top[r] = -inf;
     sum[r] = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
+    for (int g = 0; g < SG; ++g)
       low[r][g] = 0.0f;
-      o[r][2 * g] = o[r][2 * g + 1] = v4f{0, 0, 0, 0};
-    }
+#pragma unroll
+    for (int g = 0; g < 2 * G; ++g)
+      o[r][g] = v4f{0, 0, 0, 0};
   }
 
-  for (int t = tile + wave; t < tile + tiles; t += kWaves) {
-    const int key0 = t * 32;
-    bool whole = key0 >= all_lo && key0 + 32 <= all_hi;
+  // Where the wave's keys lie: lane l knows the cache's row of the first of 16
+  // keys, half l % 2 of the wave's tile l / 2 from `known_from` on.  (There are
+  // fewer than 2^32 rows: the smallest take 40 bytes twice.)
+  constexpr unsigned kNowhere = ~0u;
+  unsigned place = kNowhere;
+  int known_from = 0;
+  auto find_places = [&](int from) {
+    known_from = from;
+    const int key = (tile + kWaves * (from + (lane >> 1))) * 32 + 16 * (lane & 1);
+    place = kNowhere;
+    if (key < capacity) {
+      unsigned page = (unsigned)b, slot = (unsigned)key;
+      if (p.c.table) {
+        const unsigned at = (unsigned)key / page_size;
+        page = (unsigned)p.c.table[b * p.c.table_pages + at];
+        slot = (unsigned)key - at * page_size;
+      }
+      if (page < (uint64_t)p.c.pages)
+        place = (page * (unsigned)p.c.H + (unsigned)head) * page_size + slot;
+    }
+  };
+
+  // Codes and scales of 32 keys, as they lie: of keys c of each 16, the quarter h
+  // of the row; of keys 4 h + i, bytes c G .. of the values' rows.  Descriptors
+  // cover what the page holds of the 16 keys, nothing of a page that is none.
+  struct Tile {
+    unsigned k[2][G], v[2][4][(G + 3) / 4], ks[2][4][SG], vs[2][4][SG];
     bool known[2];
-    unsigned kw[2][4][G], vw[2][4][(G + 3) / 4];
-    v2h ks[2][4][G], vs[2][4][G];
+  };
+  const int k_at = c * (16 * G) + h * (4 * G);
+  const int v_at = 4 * h * (16 * G) + c * G, s_at = 4 * h * (4 * G) + 4 * my_group;
+  auto load = [&](Tile &t, int j) {
+    if (j - known_from >= 32)
+      find_places(j);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const Place at = place_of(p.c, b, head, key0 + 16 * u < capacity ? key0 + 16 * u : 0);
-      known[u] = at.known;
-      whole = whole && at.known;
-      const int mine = c < at.last ? c : at.last;
-      unsigned w[G];
-      load_bytes<4 * G, 4 * (G & -G) < 16 ? 4 * (G & -G) : 16>(
-          p.c.k_codes + at.row * (16 * G) + mine * (16 * G) + h * (4 * G), w);
+      const unsigned found = __builtin_amdgcn_readlane(place, 2 * (j - known_from) + u);
+      const bool known = found != kNowhere;
+      t.known[u] = known;
+      const int64_t row = known ? found : 0;
+      int room = capacity - ((tile + kWaves * j) * 32 + 16 * u);
+      room = !known ? 0 : room < 16 ? room : 16; // (whole pages hold all 16)
+      auto part = [&](const void *base, int row_bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(
+            (void *)((const char *)base + row * row_bytes), 0, room * row_bytes, 0x00020000);
+      };
+      const auto kc = part(p.c.k_codes, 16 * G), vc = part(p.c.v_codes, 16 * G);
+      const auto kp = part(p.c.k_scales, 4 * G), vp = part(p.c.v_scales, 4 * G);
+      load_words<G>(kc, k_at, t.k[u]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
+        load_words<SG>(kp, s_at + i * (4 * G), t.ks[u][i]);
 #pragma unroll
-        for (int j = 0; j < G; ++j)
-          kw[u][i][j] = w[j];
+      for (int i = 0; i < 4; ++i)
+        load_bytes<G>(vc, v_at + i * (16 * G), t.v[u][i]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 4 * h + i < at.last ? 4 * h + i : at.last;
-        load_bytes<G, (G & -G)>(p.c.v_codes + at.row * (16 * G) + key * (16 * G) + c * G, vw[u][i]);
-        const unsigned *const ka = (const unsigned *)p.c.k_scales + at.row * G + key * G;
-        const unsigned *const va = (const unsigned *)p.c.v_scales + at.row * G + key * G;
-        const Pack<unsigned, G & -G> *const kp = (const Pack<unsigned, G & -G> *)ka;
-        const Pack<unsigned, G & -G> *const vp = (const Pack<unsigned, G & -G> *)va;
-#pragma unroll
-        for (int g = 0; g < G; g += G & -G) {
-          const Pack<unsigned, G & -G> a = kp[g / (G & -G)], bb = vp[g / (G & -G)];
-#pragma unroll
-          for (int j = 0; j < (G & -G); ++j) {
-            ks[u][i][g + j] = __builtin_bit_cast(v2h, a.v[j]);
-            vs[u][i][g + j] = __builtin_bit_cast(v2h, bb.v[j]);
-          }
-        }
-      }
+      for (int i = 0; i < 4; ++i)
+        load_words<SG>(vp, s_at + i * (4 * G), t.vs[u][i]);
     }
+  };
+  auto halves = [](unsigned w) { return __builtin_bit_cast(v2h, w); };
 
+  // masked: some rows do not see some of the keys.
+  auto step_on = [&](const Tile &t, int key0, auto masked) {
     // scores, in powers of two
     float s[RT][8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       unsigned codes[G];
-      bytes_of<G, G>(kw[u], codes);
-      float part[RT][4];
+      const unsigned *const w[4] = {t.k[u], t.k[u], t.k[u], t.k[u]};
+      bytes_of<G, G, G>(w, codes);
+      v4f acc[RT][SG];
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          part[r][i] = 0.0f;
+        for (int g = 0; g < SG; ++g)
+          acc[r][g] = v4f{0, 0, 0, 0};
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         v2bf n0, n1, n2, n3;
@@ -383,32 +472,35 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
         numbers(codes[g] >> 4 & 0x0F0F0F0Fu, n2, n3);
         const v8bf k = join(n0, n1, n2, n3);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          v4f acc = {0, 0, 0, 0};
+        for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int e = TQ - 1; e >= 0; --e)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[r][g][e], acc, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            part[r][i] = __builtin_fmaf((float)ks[u][i][g][0], acc[i], part[r][i]);
-            part[r][i] = __builtin_fmaf((float)ks[u][i][g][1], qsum[r][g], part[r][i]);
-          }
-        }
+            acc[r][PACKED ? 0 : g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                k, q[r][g][e], acc[r][PACKED ? 0 : g], 0, 0, 0);
       }
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[r][4 * u + i] = part[r][i] * scale;
+        for (int i = 0; i < 4; ++i) {
+          float part = 0.0f;
+#pragma unroll
+          for (int g = 0; g < SG; ++g) {
+            const v2h pair = halves(t.ks[u][i][g]);
+            part = __builtin_fmaf((float)pair[0], acc[r][g][i], part);
+            part = __builtin_fmaf((float)pair[1], qsum[r][g], part);
+          }
+          s[r][4 * u + i] = (PACKED ? columns_sum<G>(part) : part) * scale;
+        }
     }
-    if (!whole) {
+    bool seen[RT][8];
+    if (masked.value) {
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = key0 + 16 * (j / 4) + 4 * h + j % 4;
-          if (!(known[j / 4] && key >= row_lo[r] && key < row_hi[r]))
-            s[r][j] = -inf;
+          seen[r][j] = t.known[j / 4] && key >= row_lo[r] && key < row_hi[r];
+          s[r][j] = seen[r][j] ? s[r][j] : -inf;
         }
     }
 
@@ -433,11 +525,11 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
         top[r] = m;
         sum[r] *= less;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < SG; ++g)
           low[r][g] *= less;
-          o[r][2 * g] *= less;
-          o[r][2 * g + 1] *= less;
-        }
+#pragma unroll
+        for (int g = 0; g < 2 * G; ++g)
+          o[r][g] *= less;
       }
     }
 #pragma unroll
@@ -450,10 +542,32 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
       }
     }
 
-    // output
+    // output: scaled weights, then their products
+    v8bf ps[RT][SG][TP];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const v2h pair = halves(t.vs[j / 4][j % 4][g]);
+          float vscale = (float)pair[0], vlow = (float)pair[1];
+          if (masked.value) { // nothing of a key that is not seen
+            vscale = seen[r][j] ? vscale : 0.0f;
+            vlow = seen[r][j] ? vlow : 0.0f;
+          }
+          x[j] = s[r][j] * vscale;
+          low[r][g] = __builtin_fmaf(s[r][j], vlow, low[r][g]);
+        }
+        terms_of<TP>(x, ps[r][g]);
+      }
     unsigned codes[2][G];
-    bytes_of<G, 0>(vw[0], codes[0]);
-    bytes_of<G, 0>(vw[1], codes[1]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const unsigned *const w[4] = {t.v[u][0], t.v[u][1], t.v[u][2], t.v[u][3]};
+      bytes_of<G, 0, (G + 3) / 4>(w, codes[u]);
+    }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       v2bf n0, n1, n2, n3, n4, n5, n6, n7;
@@ -463,116 +577,130 @@ __global__ __launch_bounds__(kWaves * 64) void k_cache_attention(const Arguments
       numbers(codes[1][g] >> 4 & 0x0F0F0F0Fu, n6, n7);
       const v8bf even = join(n0, n1, n2, n3), odd = join(n4, n5, n6, n7);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float ps[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const v2h pair = vs[j / 4][j % 4][g];
-          float vscale = (float)pair[0], vlow = (float)pair[1];
-          if (!whole && s[r][j] == 0.0f) // nothing of a key that is not seen
-            vscale = vlow = 0.0f;
-          ps[j] = s[r][j] * vscale;
-          low[r][g] = __builtin_fmaf(s[r][j], vlow, low[r][g]);
-        }
-        v8bf t[TP];
-        terms_of<TP>(ps, t);
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int e = TP - 1; e >= 0; --e) {
-          o[r][2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, t[e], o[r][2 * g], 0, 0, 0);
-          o[r][2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, t[e], o[r][2 * g + 1], 0, 0, 0);
+          const v8bf w = ps[r][PACKED ? 0 : g][e];
+          o[r][2 * g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, w, o[r][2 * g], 0, 0, 0);
+          o[r][2 * g + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, w, o[r][2 * g + 1], 0, 0, 0);
         }
+    }
+  };
+
+  auto step = [&](const Tile &t, int j) {
+    const int key0 = (tile + kWaves * j) * 32;
+    if (key0 >= all_lo && key0 + 32 <= all_hi && t.known[0] && t.known[1])
+      step_on(t, key0, std::false_type{});
+    else
+      step_on(t, key0, std::true_type{});
+  };
+
+  // The next tile is on its way while one is worked on; 16 rows a tile leave no
+  // registers for that (their scales alone are 16 G of them).
+  if (tiles > 0)
+    find_places(0);
+  if constexpr (PACKED) {
+    Tile one, other;
+    if (tiles > 0)
+      load(one, 0);
+    for (int j = 0; j < tiles; j += 2) {
+      load(other, j + 1 < tiles ? j + 1 : j);
+      step(one, j);
+      if (j + 1 < tiles) {
+        load(one, j + 2 < tiles ? j + 2 : j + 1);
+        step(other, j + 1);
       }
+    }
+  } else {
+    for (int j = 0; j < tiles; ++j) {
+      Tile one;
+      load(one, j);
+      step(one, j);
     }
   }
 
-  // The waves' results meet in LDS: [wave][g][lane][8] output, then (max, sum).
-  float *const stats = shared + kWaves * G * 64 * 8;
-#pragma unroll 1
+  // The waves' results meet in LDS: [wave][g][h][row][8] output, then (max, sum).
+  constexpr int kPiece = 4 * ROWS * 8;
+  float *const stats = shared + kWaves * G * kPiece;
+#pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float my_top = 0, my_sum = 0;
+    float all = sum[r];
+    all += __shfl_xor(all, 16);
+    all += __shfl_xor(all, 32);
 #pragma unroll
-    for (int k = 0; k < RT; ++k) {
-      if (k != r)
-        continue;
-      my_top = top[k];
-      my_sum = sum[k];
-      my_sum += __shfl_xor(my_sum, 16);
-      my_sum += __shfl_xor(my_sum, 32);
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        float l = low[k][g];
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        float *const to = shared + ((wave * G + g) * 64 + lane) * 8;
-        const v4f e = o[k][2 * g] + l, f = o[k][2 * g + 1] + l;
+    for (int g = 0; g < G; ++g) {
+      float l = low[r][PACKED ? 0 : g];
+      l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      if (!PACKED || g == my_group) {
+        float *const to = shared + (wave * G + g) * kPiece + (h * ROWS + my_row) * 8;
+        const v4f e = o[r][2 * g] + l, f = o[r][2 * g + 1] + l;
         *(v4f *)to = v4f{e[0], f[0], e[1], f[1]};
         *(v4f *)(to + 4) = v4f{e[2], f[2], e[3], f[3]};
       }
     }
-    if (h == 0) {
-      stats[(wave * 16 + c) * 2] = my_top;
-      stats[(wave * 16 + c) * 2 + 1] = my_sum;
+    if (lane < ROWS) {
+      stats[(wave * ROWS + lane) * 2] = top[r];
+      stats[(wave * ROWS + lane) * 2 + 1] = all;
     }
     __syncthreads();
-    const int row = row0 + 16 * r + c;
-    float m = -inf, total = 0.0f, factor[kWaves];
+    // Pieces of 8 elements: (g, quarter, row).
+    for (int at = threadIdx.x; at < G * 4 * ROWS; at += kWaves * 64) {
+      const int mr = at % ROWS, g = at / (4 * ROWS), quarter = at / ROWS % 4;
+      const int row = row0 + ROWS * r + mr;
+      if (row >= rows)
+        continue;
+      float m = -inf, total = 0.0f, v[8];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      m = __builtin_fmaxf(m, stats[(w * 16 + c) * 2]);
+      for (int j = 0; j < 8; ++j)
+        v[j] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float mw = stats[(w * 16 + c) * 2];
-      factor[w] = mw == -inf ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
-      total += stats[(w * 16 + c) * 2 + 1] * factor[w];
-    }
-    if (row < rows) {
-      const int64_t part = ((int64_t)unit * p.splits + split) * (RT * 16) + 16 * r + c;
-      const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
-      const int64_t at = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
-                                       : ((int64_t)b * p.S + i) * p.heads + qh;
-      for (int g = wave; g < G; g += kWaves) {
-        float v[8];
+      for (int w = 0; w < kWaves; ++w)
+        m = __builtin_fmaxf(m, stats[(w * ROWS + mr) * 2]);
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float mw = stats[(w * ROWS + mr) * 2];
+        const float f = mw == -inf ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+        total += stats[(w * ROWS + mr) * 2 + 1] * f;
+        const float *const from = shared + w * G * kPiece + at * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          v[j] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          const float *const from = shared + ((w * G + g) * 64 + lane) * 8;
-          // (a wave without keys holds zeros)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[j] = __builtin_fmaf(from[j], factor[w], v[j]);
-        }
-        if (p.splits == 1) {
-          const float over = total == 0.0f ? 0.0f : 1.0f / total;
-          T *const y = (T *)p.y + at * D + 32 * g + 8 * h;
-          Pack<T, 8> out;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            out.v[j] = from_f32<T>(v[j] * over);
-          *(Pack<T, 8> *)y = out;
-        } else {
-          float *const y = p.parts + part * D + 32 * g + 8 * h;
-          *(v4f *)y = v4f{v[0], v[1], v[2], v[3]};
-          *(v4f *)(y + 4) = v4f{v[4], v[5], v[6], v[7]};
-        }
+          v[j] = __builtin_fmaf(from[j], f, v[j]);
       }
-      if (p.splits > 1 && wave == 0 && h == 0) {
-        float *const st = p.parts + (int64_t)p.B * p.c.H * p.groups * p.splits * (RT * 16) * D + part * 2;
-        st[0] = m;
-        st[1] = total;
+      if (p.splits == 1) {
+        const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
+        const int64_t to = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
+                                         : ((int64_t)b * p.S + i) * p.heads + qh;
+        const float over = total == 0.0f ? 0.0f : 1.0f / total;
+        Pack<T, 8> out;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          out.v[j] = from_f32<T>(v[j] * over);
+        *(Pack<T, 8> *)((T *)p.y + to * D + 32 * g + 8 * quarter) = out;
+      } else {
+        const int64_t part = ((int64_t)unit * p.splits + split) * (RT * ROWS) + ROWS * r + mr;
+        float *const y = p.parts + part * D + 32 * g + 8 * quarter;
+        *(v4f *)y = v4f{v[0], v[1], v[2], v[3]};
+        *(v4f *)(y + 4) = v4f{v[4], v[5], v[6], v[7]};
+        if (g == 0 && quarter == 0) {
+          float *const st = p.parts +
+              (int64_t)p.B * p.c.H * p.groups * p.splits * (RT * ROWS) * D + part * 2;
+          st[0] = m;
+          st[1] = total;
+        }
       }
     }
     __syncthreads();
   }
 }
 
-// The parts of a row's keys joined: thread (s, d) sums every 8th part's
-// elements 4 d .., and the eight sums meet in LDS.
+// The parts of a row's keys joined, a block a row: thread t weighs part t (there
+// are at most 256), then thread (s, d) sums elements 4 d .. of every part s, s +
+// across, .., and those sums meet in LDS.
 template <typename T>
 __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, int tile_rows) {
-  extern __shared__ __attribute__((aligned(16))) float shared[];
-  const int lanes = D / 4, across = 256 / lanes; // threads of a row, parts at once
+  __shared__ float weight[256], tops[4], sums[4];
+  __shared__ __attribute__((aligned(16))) float pieces[256 * 4];
   const int unit = blockIdx.x / tile_rows, r = blockIdx.x % tile_rows;
   const int group = unit % p.groups, bh = unit / p.groups;
   const int b = bh / p.c.H, head = bh % p.c.H;
@@ -584,34 +712,42 @@ __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, in
   const int row = group * tile_rows + r;
   if (row >= count * p.per_head)
     return;
+  const int t = threadIdx.x;
+  const int lanes = D / 4, across = 256 / lanes; // threads of a row, parts at once
   const float inf = __builtin_inff();
   const float *const stats = p.parts + (int64_t)p.B * p.c.H * p.groups * p.splits * tile_rows * D;
   const int64_t part0 = (int64_t)unit * p.splits * tile_rows + r;
-  const int s0 = threadIdx.x / lanes, d = threadIdx.x % lanes;
-  float m = -inf;
-  for (int s = 0; s < p.splits; ++s)
-    m = __builtin_fmaxf(m, stats[(part0 + (int64_t)s * tile_rows) * 2]);
+  float m = -inf, total = 0.0f;
+  if (t < p.splits) {
+    m = stats[(part0 + (int64_t)t * tile_rows) * 2];
+    total = stats[(part0 + (int64_t)t * tile_rows) * 2 + 1];
+  }
+  auto over_block = [&](float v, float (&of)[4], auto fold) {
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2)
+      v = fold(v, __shfl_xor(v, i));
+    if (t % 64 == 0)
+      of[t / 64] = v;
+    __syncthreads();
+    return fold(fold(of[0], of[1]), fold(of[2], of[3]));
+  };
+  const float top = over_block(m, tops, [](float x, float y) { return __builtin_fmaxf(x, y); });
+  const float f = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+  weight[t] = f;
+  total = over_block(total * f, sums, [](float x, float y) { return x + y; });
+  const int s0 = t / lanes, d = t % lanes;
   v4f v = {0, 0, 0, 0};
-  float total = 0.0f;
-  if (s0 < across)
-    for (int s = s0; s < p.splits; s += across) {
-      const int64_t part = part0 + (int64_t)s * tile_rows;
-      const float ms = stats[part * 2];
-      const float f = ms == -inf ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
-      total += stats[part * 2 + 1] * f;
-      v += *(const v4f *)(p.parts + part * D + 4 * d) * f;
-    }
-  float *const mine = shared + threadIdx.x * 8;
-  *(v4f *)mine = v;
-  mine[4] = total;
+  if (s0 < across) {
+#pragma unroll 4
+    for (int s = s0; s < p.splits; s += across)
+      v += *(const v4f *)(p.parts + (part0 + (int64_t)s * tile_rows) * D + 4 * d) * weight[s];
+  }
+  *(v4f *)(pieces + 4 * t) = v;
   __syncthreads();
   if (s0 > 0)
     return;
-  for (int s = 1; s < across; ++s) {
-    const float *const other = shared + (s * lanes + d) * 8;
-    v += *(const v4f *)other;
-    total += other[4];
-  }
+  for (int s = 1; s < across; ++s)
+    v += *(const v4f *)(pieces + 4 * (s * lanes + d));
   const float over = total == 0.0f ? 0.0f : 1.0f / total;
   const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
   const int64_t at = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
@@ -623,18 +759,30 @@ __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, in
   *(Pack<T, 4> *)((T *)p.y + at * D + 4 * d) = out;
 }
 
-int row_tiles(const Attention4 &a) {
-  return a.S * (a.heads / a.c.H) > 16 && a.c.D <= 128 ? 2 : 1;
+// How rows are dealt to waves: tiles of 16, or of 16 / G where that takes one
+// tile (D = 64, 128, 256) or two (64, 128).
+struct Shape {
+  bool packed;
+  int tiles, rows; // tiles of a wave; rows of a tile
+};
+Shape shape_of(const Attention4 &a) {
+  const int64_t n = a.S * (a.heads / a.c.H);
+  const int G = a.c.D / kCacheGroup;
+  if (16 % G == 0 && n <= (G <= 4 ? 2 : 1) * (16 / G))
+    return {true, n > 16 / G ? 2 : 1, 16 / G};
+  return {false, n > 16 && G <= 4 ? 2 : 1, 16};
 }
 int64_t row_groups(const Attention4 &a) {
-  const int rows = 16 * row_tiles(a);
+  const Shape s = shape_of(a);
+  const int rows = s.rows * s.tiles;
   return (a.S * (a.heads / a.c.H) + rows - 1) / rows;
 }
 
-template <typename T, int G, int RT>
+template <typename T, int G, int RT, bool PACKED>
 hipError_t attend(hipStream_t st, const Arguments &p) {
-  constexpr int kLds = (kWaves * G * 64 * 8 + kWaves * 16 * 2) * 4;
-  auto *const kernel = k_cache_attention<T, G, RT>;
+  constexpr int kRows = PACKED ? 16 / G : 16;
+  constexpr int kLds = (kWaves * G * 4 * kRows * 8 + kWaves * kRows * 2) * 4;
+  auto *const kernel = k_cache_attention<T, G, RT, PACKED>;
   if (kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void *)kernel,
         hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
@@ -645,25 +793,43 @@ hipError_t attend(hipStream_t st, const Arguments &p) {
   kernel<<<dim3((unsigned)(units * p.splits)), kWaves * 64, kLds, st>>>(p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.splits > 1) {
-    k_cache_join<T><<<dim3((unsigned)(units * RT * 16)), 256, 256 * 8 * 4, st>>>(p, 32 * G, RT * 16);
+    k_cache_join<T><<<dim3((unsigned)(units * RT * kRows)), 256, 0, st>>>(
+        p, 32 * G, RT * kRows);
     e = hipGetLastError();
   }
   return e;
 }
 
+template <typename T, int G>
+hipError_t attend_group(hipStream_t st, const Arguments &p, const Shape &s) {
+  if constexpr (16 % G == 0) {
+    if (s.packed && s.tiles == 1)
+      return attend<T, G, 1, true>(st, p);
+  }
+  if constexpr (G <= 4) {
+    if constexpr (16 % G == 0) {
+      if (s.packed)
+        return attend<T, G, 2, true>(st, p);
+    }
+    if (s.tiles > 1)
+      return attend<T, G, 2, false>(st, p);
+  }
+  return attend<T, G, 1, false>(st, p);
+}
+
 template <typename T>
-hipError_t attend_any(hipStream_t st, const Arguments &p, int tiles) {
+hipError_t attend_any(hipStream_t st, const Arguments &p, const Shape &s) {
   switch (p.c.D / kCacheGroup) {
   case 2:
-    return tiles > 1 ? attend<T, 2, 2>(st, p) : attend<T, 2, 1>(st, p);
+    return attend_group<T, 2>(st, p, s);
   case 3:
-    return tiles > 1 ? attend<T, 3, 2>(st, p) : attend<T, 3, 1>(st, p);
+    return attend_group<T, 3>(st, p, s);
   case 4:
-    return tiles > 1 ? attend<T, 4, 2>(st, p) : attend<T, 4, 1>(st, p);
+    return attend_group<T, 4>(st, p, s);
   case 6:
-    return attend<T, 6, 1>(st, p);
+    return attend_group<T, 6>(st, p, s);
   default:
-    return attend<T, 8, 1>(st, p);
+    return attend_group<T, 8>(st, p, s);
   }
 }
 
@@ -710,19 +876,22 @@ hipError_t launch_cache_append(hipStream_t s, const Append4 &a) {
   }
 }
 
-// Parts of the keys, so that a few rows fill the GPU: about four blocks a CU,
-// of 128 keys at least.  (How many keys there are, only the GPU knows: a block
-// takes its share of what its rows see.)
+// Parts of the keys, so that a few rows fill the GPU: two blocks a CU, which is
+// what its registers hold, of 128 keys at least.  (How many keys there are, only
+// the GPU knows: a block takes its share of what its rows see.)  131072 keys, 8
+// heads of 128, in parts for 256 / 512 / 768 / 1024 / 2048 blocks: 42 / 44 / 48 /
+// 53 / 64 us; 32 sequences of 2000 - 4000 keys 38 / 37 / 43 / 44 / 58.
 int attention_splits(const Attention4 &a) {
   const int64_t units = a.B * a.c.H * row_groups(a);
   const int64_t capacity = a.c.table ? a.c.table_pages * a.c.page_size : a.c.page_size;
-  int64_t n = 1024 / (units > 0 ? units : 1);
+  int64_t n = 512 / (units > 0 ? units : 1);
   if (n > (capacity + 127) / 128)
     n = (capacity + 127) / 128;
   return (int)(n < 1 ? 1 : n < 256 ? n : 256);
 }
 size_t attention_parts_bytes(const Attention4 &a) {
-  const int64_t rows = a.B * a.c.H * row_groups(a) * 16 * row_tiles(a);
+  const Shape shape = shape_of(a);
+  const int64_t rows = a.B * a.c.H * row_groups(a) * shape.rows * shape.tiles;
   return (size_t)rows * a.splits * (a.c.D + 2) * sizeof(float);
 }
 
@@ -732,11 +901,11 @@ hipError_t launch_cache_attention(hipStream_t s, const Attention4 &a) {
       a.causal, a.heads_first};
   switch (a.kind) {
   case kF32:
-    return attend_any<float>(s, p, row_tiles(a));
+    return attend_any<float>(s, p, shape_of(a));
   case kF16:
-    return attend_any<_Float16>(s, p, row_tiles(a));
+    return attend_any<_Float16>(s, p, shape_of(a));
   default:
-    return attend_any<__bf16>(s, p, row_tiles(a));
+    return attend_any<__bf16>(s, p, shape_of(a));
   }
 }
 
