@@ -235,6 +235,24 @@ __device__ __forceinline__ v8bf widen8(unsigned w0, unsigned w1) {
   return v8bf{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// The operands of the four instructions of a block of 128, from a lane's bytes of
+// either half of it.
+__device__ __forceinline__ void widen16(v4u l, v4u u, v8bf (&w)[4]) {
+  w[0] = widen8(l[0], l[1]);
+  w[1] = widen8(l[2], l[3]);
+  w[2] = widen8(u[0], u[1]);
+  w[3] = widen8(u[2], u[3]);
+}
+__device__ __forceinline__ v8i operand(v4u l, v4u u) {
+  return v8i{(int)l[0], (int)l[1], (int)l[2], (int)l[3], (int)u[0], (int)u[1],
+      (int)u[2], (int)u[3]};
+}
+__device__ __forceinline__ void add_scaled(float (&total)[4], v4f acc, float s) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    total[r] = __builtin_fmaf(acc[r], s, total[r]);
+}
+
 struct GemmParams {
   const uint8_t *a, *b;
   const float *a_scale, *b_scale, *bias;
@@ -244,6 +262,10 @@ struct GemmParams {
   int kblocks;       // scales of a row: ceil(K / 128) of the caller's K
   int bias_step;     // 0: one bias for all columns
   int activation;
+  int parts;         // of the blocks of K, part_blocks each
+  int part_blocks;
+  int part_pitch;    // N, rounded up to whole pieces of four
+  float *part_sums;  // [parts, M, part_pitch] if parts > 1
 };
 
 __device__ __forceinline__ float finish(float v, const GemmParams &p, float bias) {
@@ -255,10 +277,16 @@ __device__ __forceinline__ float finish(float v, const GemmParams &p, float bias
   return v;
 }
 
+// Whether rows of y divide into aligned pieces of n elements.
+template <typename T>
+__device__ __forceinline__ bool whole_pieces(const GemmParams &p, int n) {
+  return p.N % n == 0 && (uintptr_t)p.y % (n * sizeof(T)) == 0;
+}
+
 // Four neighbouring columns n .. n + 3 of row m; those past N are left out.
 template <typename T>
 __device__ __forceinline__ void store4(
-    const GemmParams &p, int m, int n, const float (&v)[4], bool whole) {
+    const GemmParams &p, int m, int n, const float (&v)[4]) {
   T *const y = (T *)p.y + (int64_t)m * p.N + n;
   T t[4];
 #pragma unroll
@@ -267,7 +295,7 @@ __device__ __forceinline__ void store4(
     const float bias = p.bias ? p.bias[c * p.bias_step] : 0.0f;
     t[i] = from_f32<T>(finish(v[i], p, bias));
   }
-  if (whole && n + 4 <= p.N) {
+  if (whole_pieces<T>(p, 4) && n + 4 <= p.N) {
     *(Pack<T, 4> *)y = *(const Pack<T, 4> *)t;
   } else {
 #pragma unroll
@@ -389,24 +417,34 @@ __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p)
       t += *(const v4f *)sums[w][i][lane];
     const float v[4] = {t[0], t[1], t[2], t[3]};
     if (16 * i + c < p.M)
-      store4<T>(p, 16 * i + c, n0 + 4 * h, v, p.N % 4 == 0);
+      store4<T>(p, 16 * i + c, n0 + 4 * h, v);
   }
+}
+
+// 16 bytes a lane from `from` + at + k (k the same in all lanes; nothing from
+// `bytes` on) into LDS, the wave's from `to` on, one after the other.
+__device__ __forceinline__ void copy16(
+    const void *from, void *to, int at, int k, unsigned bytes = 0x7FFFFFFF) {
+  typedef __attribute__((address_space(3))) void *lds_ptr;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, bytes, 0x00020000),
+      (lds_ptr)to, 16, at, k, 0, 0);
 }
 
 // --- tiles ------------------------------------------------------------------
 // BM x BN tiles, WM x WN waves.  A step is one block of 128 of K: the rows'
-// 128 bytes go straight into LDS (two stages), 16-byte chunk q of row r at
+// 128 bytes go straight into LDS (two or three stages), 16-byte chunk q of row r at
 // place q ^ (r % 8), so that neither the copies nor the operand reads meet a
 // bank twice.  Columns are the first operand of the matrix instruction, so a
 // lane holds one row of the result and four neighbouring columns: one scale
-// for all it gets from an instruction, and whole pieces to store.
-template <typename T, int BM, int BN, int WM, int WN, bool EXACT>
-__global__ __launch_bounds__(WM * WN * 64) void k_block_tile(const GemmParams p) {
+// for all it gets from an instruction, and whole pieces to store.  A part of
+// the blocks of K (parts > 1) leaves f32 sums for k_join_parts.
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool EXACT>
+__global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams p) {
   constexpr int THREADS = WM * WN * 64, STAGE = (BM + BN) * kBlock;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   constexpr int COPIES = STAGE / (THREADS * 16); // of 16 bytes a thread
-  static_assert(BN % kBlock == 0 || kBlock % BN == 0, "one scale a tile's columns");
-  static_assert(STAGE % (THREADS * 16) == 0, "copies");
+  static_assert(STAGE % (THREADS * 16) == 0 && BM * 8 % THREADS == 0, "copies");
   extern __shared__ __attribute__((aligned(16))) uint8_t sm[];
 
   const int lane = threadIdx.x & 63;
@@ -415,59 +453,77 @@ __global__ __launch_bounds__(WM * WN * 64) void k_block_tile(const GemmParams p)
   const int wm = wave / WN, wn = wave % WN;
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   // Neighbouring blocks of an XCD share rows of a and of b in its L2.
-  const int id = xcd_contiguous(blockIdx.x, tiles_m * tiles_n);
+  int id = xcd_contiguous(blockIdx.x, tiles_m * tiles_n * p.parts);
+  const int part = id / (tiles_m * tiles_n);
+  id -= part * (tiles_m * tiles_n);
   constexpr int GROUP = 8;
   const int first = id / (GROUP * tiles_n) * GROUP;
   const int span = tiles_m - first < GROUP ? tiles_m - first : GROUP;
   const int m0 = (first + id % (GROUP * tiles_n) % span) * BM;
   const int n0 = id % (GROUP * tiles_n) / span * BN;
+  const int kb0 = part * p.part_blocks;
+  const int kb1 = kb0 + p.part_blocks < p.kblocks ? kb0 + p.part_blocks : p.kblocks;
 
   // Copies: thread t's piece j is chunk t % 8 of row (t + j THREADS) / 8 of the
-  // stage, rows of a first.  Rows past the matrix repeat its last one.
-  typedef __attribute__((address_space(3))) void *lds_ptr;
-  typedef const __attribute__((address_space(1))) void *glb_ptr;
-  const uint8_t *from[COPIES];
+  // stage, rows of a first, by descriptors that begin at the tile's rows.  Rows
+  // past the matrix repeat its last one.
+  const int chunk = (threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7);
+  static_assert(THREADS / 8 % 8 == 0, "a thread's pieces have one place in their rows");
+  const uint8_t *const a0 = p.a + (int64_t)m0 * p.lda;
+  const uint8_t *const b0 = p.b + (int64_t)n0 * p.ldb;
+  int from[COPIES];
 #pragma unroll
   for (int j = 0; j < COPIES; ++j) {
     const int r = ((int)threadIdx.x + j * THREADS) / 8;
-    const int q = (threadIdx.x & 7) ^ (r & 7);
-    if (j * THREADS / 8 < BM) {
-      const int m = m0 + r < p.M ? m0 + r : p.M - 1;
-      from[j] = p.a + (int64_t)m * p.lda + 16 * q;
-    } else {
-      const int n = n0 + r - BM < p.N ? n0 + r - BM : p.N - 1;
-      from[j] = p.b + (int64_t)n * p.ldb + 16 * q;
-    }
+    if (j * THREADS / 8 < BM)
+      from[j] = (m0 + r < p.M ? r : p.M - 1 - m0) * p.lda + 16 * chunk;
+    else
+      from[j] = (n0 + r - BM < p.N ? r - BM : p.N - 1 - n0) * p.ldb + 16 * chunk;
   }
-  static_assert(BM * 8 % THREADS == 0, "a copy is of one operand");
-  auto copy = [&](int kb, int stage) {
+  // Pieces j0 .. j1 - 1 of a step's copies.
+  auto copy = [&](int kb, int stage, int j0, int j1) {
     const int k = kb * kBlock;
+    // (in the last block: chunks past the row's end come from its last one and
+    // are cleared below)
+    const int left = p.K - k;
+    const int back = 16 * (chunk + 1) > left ? 16 * (chunk + 1) - left : 0;
+    uint8_t *const to = sm + stage * STAGE + wave * 1024;
 #pragma unroll
-    for (int j = 0; j < COPIES; ++j) {
-      uint8_t *const to = sm + stage * STAGE + j * THREADS * 16 + wave * 1024;
-      // (in the last block: chunks past the row's end come from its last one
-      // and are cleared below)
-      const int over = k + kBlock > p.K ? k + kBlock - p.K : 0;
-      const int q = ((threadIdx.x & 7) ^ ((((int)threadIdx.x + j * THREADS) / 8) & 7));
-      const int back = over && 16 * (q + 1) > kBlock - over ? 16 * (q + 1) - (kBlock - over) : 0;
-      __builtin_amdgcn_global_load_lds((glb_ptr)(from[j] + k - back), (lds_ptr)to, 16, 0, 0);
-    }
+    for (int j = j0; j < j1; ++j)
+      copy16(j * THREADS / 8 < BM ? a0 : b0, to + j * THREADS * 16, from[j] - back, k);
   };
 
-  // Scales: one a row of the result and step, and one for all columns.
-  const float *as[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + (wm * TM + i) * 16 + c;
-    as[i] = p.a_scale + (int64_t)(m < p.M ? m : p.M - 1) * p.kblocks;
+  // Scales, one for each row and one for 128 columns, come four steps at a time, 16
+  // bytes a row, 64 rows a wave: waves 0 .. BM / 64 - 1 those of the rows, the next
+  // the columns', the others nothing that is read.  A CU has some 64 requests to
+  // L2 on their way, each a line at most, and a scale by itself is one: a step's
+  // 256 + 256 rows are 512, their scales one by one were 260 more (256 x 256 tiles,
+  // 8192x8192x8192 530 us; every wave fetching its own 16 rows' 1170).
+  constexpr int WAVES = WM * WN, NB = (BN + 2 * kBlock - 2) / kBlock; // columns' blocks
+  constexpr int SET = WAVES * 256; // floats of four steps' scales
+  static_assert(BM % 64 == 0 && WAVES > BM / 64 && NB <= 64, "a wave for the columns' scales");
+  float *const scales = (float *)(sm + STAGES * STAGE); // [2][WAVES][64][4]
+  const float *scale0 = p.a_scale + (int64_t)m0 * p.kblocks;
+  int scale_at;
+  unsigned scale_bytes; // from scale0 on
+  {
+    const int m = wave * 64 + lane, last = (p.N - 1) / kBlock;
+    const int n = n0 / kBlock + (lane < NB ? lane : 0);
+    int64_t rows_left = (int64_t)p.M - m0;
+    if (wave < BM / 64) {
+      scale_at = (m0 + m < p.M ? m : p.M - 1 - m0) * p.kblocks * 4;
+    } else {
+      scale0 = p.b_scale + (int64_t)(n0 / kBlock) * p.kblocks;
+      scale_at = ((n < last ? n : last) - n0 / kBlock) * p.kblocks * 4;
+      rows_left = last + 1 - n0 / kBlock;
+    }
+    const int64_t bytes = rows_left * p.kblocks * 4;
+    scale_bytes = bytes < 0x7FFFFFFF ? (unsigned)bytes : 0x7FFFFFFFu;
   }
-  constexpr int NB = BN / WN > kBlock ? BN / WN / kBlock : 1; // scales of a wave's columns
-  const float *bs[NB];
-#pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int n = n0 + wn * (BN / WN) + j * kBlock;
-    bs[j] = p.b_scale + (int64_t)((n < p.N ? n : p.N - 1) / kBlock) * p.kblocks;
-  }
+  scale_bytes = __builtin_amdgcn_readfirstlane(scale_bytes);
+  auto scales_of = [&](int kb, int set) { // (of blocks kb .. kb + 3)
+    copy16(scale0, scales + set * SET + wave * 256, scale_at, kb * 4, scale_bytes);
+  };
 
   float total[TM][TN][4];
 #pragma unroll
@@ -478,27 +534,27 @@ __global__ __launch_bounds__(WM * WN * 64) void k_block_tile(const GemmParams p)
       for (int r = 0; r < 4; ++r)
         total[i][j][r] = 0.0f;
 
-  float sa[TM], sb[NB];
-  if (p.kblocks > 0) { // (no elements in a row: the sums are 0)
-    copy(0, 0);
+  // A step's memory operations of a wave: the scales of four, in every fourth step,
+  // then COPIES copies.  All but the COPIES (STAGES - 2) last having landed, the
+  // step's rows have, and its scales, which are fetched four steps before.
+  const int steps = kb1 - kb0;
+  auto step_at = [&](int i) { return kb0 + (i < steps ? i : steps - 1); };
+  if (steps > 0) { // (no elements in a row: the sums are 0)
+    scales_of(kb0, 0);
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-      sa[i] = as[i][0];
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-      sb[j] = bs[j][0];
+    for (int i = 0; i < STAGES - 1; ++i)
+      copy(step_at(i), i, 0, COPIES);
   }
-  for (int kb = 0; kb < p.kblocks; ++kb) {
-    // this step's rows are in LDS, the last step's have been read by all
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    uint8_t *const st = sm + (kb & 1) * STAGE;
-    float s[TM][NB];
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < NB; ++j)
-        s[i][j] = sa[i] * sb[j];
+  int stage = 0;
+  for (int step = 0; step < steps; ++step) {
+    // this step's rows are in LDS; those of the step before have been read by all,
+    // and the last of the steps ahead goes where they were
+    // (not __syncthreads, which waits for every copy on its way)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((STAGES - 2) * COPIES)
+                 : "memory");
+    const int kb = kb0 + step;
+    uint8_t *const st = sm + stage * STAGE;
+    const float *const sc = scales + (step >> 2 & 1) * SET + (step & 3);
     if (kb * kBlock + kBlock > p.K) { // chunks past the row's end
       const int left = (p.K - kb * kBlock) / 16;
       for (int i = threadIdx.x; i < (BM + BN) * 8; i += THREADS)
@@ -506,88 +562,175 @@ __global__ __launch_bounds__(WM * WN * 64) void k_block_tile(const GemmParams p)
           *(v4u *)(st + i * 16) = v4u{0, 0, 0, 0};
       __syncthreads();
     }
-    if (kb + 1 < p.kblocks) {
-      copy(kb + 1, (kb + 1) & 1);
+    // The copies are dealt out over the wave's rows: a wave is held at each until
+    // the path to memory has taken the one before.
+    const int ahead = step_at(step + STAGES - 1);
+    const int to_stage = stage == 0 ? STAGES - 1 : stage - 1;
+    auto copies_of = [&](int i) {
+      if (i == 0 && (step & 3) == 0)
+        scales_of(kb + 4, (step >> 2 & 1) ^ 1);
+      copy(ahead, to_stage, COPIES * i / TM, COPIES * (i + 1) / TM);
+      __builtin_amdgcn_sched_barrier(0x38F); // (only memory operations stay in place)
+    };
+    stage = stage + 1 < STAGES ? stage + 1 : 0;
+    float sa_now[TM], sb_now[TN];
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
-        sa[i] = as[i][kb + 1];
+    for (int i = 0; i < TM; ++i)
+      sa_now[i] = sc[((wm * TM + i) * 16 + c) * 4];
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        sb[j] = bs[j][kb + 1];
-    }
+    for (int j = 0; j < TN; ++j)
+      sb_now[j] = sc[(BM + (n0 % kBlock + (wn * TN + j) * 16) / kBlock) * 4];
     // lane (c, h): chunks h and h + 4 of row c of each 16
     auto read = [&](int row, int half) -> v4u {
       const int r = row + c;
       return *(const v4u *)(st + r * kBlock + (((h + 4 * half) ^ (r & 7)) << 4));
     };
-    v4u fa[TM][2];
+    // The wave's columns stay in registers, its rows pass through them.
+    auto columns = [&](int j, int half) { return read(BM + (wn * TN + j) * 16, half); };
+    auto rows = [&](int i, int half) { return read((wm * TM + i) * 16, half); };
+    if constexpr (EXACT) {
+      v8bf wb[TN][4];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+      for (int j = 0; j < TN; ++j)
+        widen16(columns(j, 0), columns(j, 1), wb[j]);
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        fa[i][half] = read((wm * TM + i) * 16, half);
-    if (EXACT) {
+      for (int i = 0; i < TM; ++i) {
+        copies_of(i);
+        v8bf wa[4];
+        widen16(rows(i, 0), rows(i, 1), wa);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        v4f acc[TM];
+        for (int j = 0; j < TN; ++j) {
+          v4f acc = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-          acc[i] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const v4u w = read(BM + (wn * TN + j) * 16, half);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const v8bf fb = widen8(w[2 * e], w[2 * e + 1]);
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-              acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb,
-                  widen8(fa[i][half][2 * e], fa[i][half][2 * e + 1]), acc[i], 0, 0, 0);
-          }
+          for (int e = 0; e < 4; ++e)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j][e], wa[e], acc, 0, 0, 0);
+          add_scaled(total[i][j], acc, sa_now[i] * sb_now[j]);
         }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            total[i][j][r] = __builtin_fmaf(
-                acc[i][r], s[i][NB > 1 ? j * 16 / kBlock : 0], total[i][j][r]);
       }
     } else {
+      v8i fb[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const v4u lo = read(BM + (wn * TN + j) * 16, 0);
-        const v4u hi = read(BM + (wn * TN + j) * 16, 1);
-        const v8i fb = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0],
-            (int)hi[1], (int)hi[2], (int)hi[3]};
-        v4f acc[TM];
+      for (int j = 0; j < TN; ++j)
+        fb[j] = operand(columns(j, 0), columns(j, 1));
+      v8i next = operand(rows(0, 0), rows(0, 1));
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          const v8i f = {(int)fa[i][0][0], (int)fa[i][0][1], (int)fa[i][0][2],
-              (int)fa[i][0][3], (int)fa[i][1][0], (int)fa[i][1][1],
-              (int)fa[i][1][2], (int)fa[i][1][3]};
-          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              fb, f, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
-        }
+      for (int i = 0; i < TM; ++i) {
+        copies_of(i);
+        const v8i fa = next;
+        if (i + 1 < TM)
+          next = operand(rows(i + 1, 0), rows(i + 1, 1));
+        v4f acc[TN];
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+        for (int j = 0; j < TN; ++j)
+          acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              fb[j], fa, v4f{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            total[i][j][r] = __builtin_fmaf(
-                acc[i][r], s[i][NB > 1 ? j * 16 / kBlock : 0], total[i][j][r]);
+        for (int j = 0; j < TN; ++j)
+          add_scaled(total[i][j], acc[j], sa_now[i] * sb_now[j]);
       }
     }
   }
+  // (the last steps have copied the last one once more)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (p.parts > 1) {
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int m = m0 + (wm * TM + i) * 16 + c;
-    if (m < p.M)
+    for (int i = 0; i < TM; ++i) {
+      const int m = m0 + (wm * TM + i) * 16 + c;
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int n = n0 + (wn * TN + j) * 16 + 4 * h;
-        if (n < p.N)
-          store4<T>(p, m, n, total[i][j], p.N % 4 == 0);
+        const float *const t = total[i][j];
+        if (m < p.M && n < p.N)
+          *(v4f *)(p.part_sums + ((int64_t)part * p.M + m) * p.part_pitch + n) =
+              v4f{t[0], t[1], t[2], t[3]};
+      }
+    }
+    return;
+  }
+  // Results leave by way of LDS, so that a store takes whole lines of rows: each
+  // wave's 16 TM x 16 TN, 16-byte chunk q of row r at place q ^ (r % 8).
+  constexpr int ROW = TN * 16 * (int)sizeof(T), CHUNKS = ROW / 16;
+  static_assert(WM * WN * TM * 16 * ROW <= STAGES * STAGE && CHUNKS <= 64, "LDS");
+  __syncthreads();
+  uint8_t *const mine = sm + wave * (TM * 16 * ROW);
+  auto place = [&](int row, int chunk) {
+    return row * ROW + ((CHUNKS % 8 == 0 ? chunk ^ (row & 7) : chunk) << 4);
+  };
+  float bias[TN][4];
+#pragma unroll
+  for (int j = 0; j < TN; ++j)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      bias[j][r] = 0.0f;
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = n0 + (wn * TN + j) * 16 + 4 * h + r;
+        bias[j][r] = p.bias[(n < p.N ? n : p.N - 1) * p.bias_step];
       }
   }
+#pragma unroll
+  for (int j = 0; j < TN; ++j) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      Pack<T, 4> out;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        total[i][j][r] += bias[j][r];
+      if (p.activation)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          total[i][j][r] = p.activation == OM_MI355X_ACTIVATION_RELU
+                               ? __builtin_fmaxf(total[i][j][r], 0.0f)
+                               : gemm::gelu_f32(total[i][j][r]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        out.v[r] = from_f32<T>(total[i][j][r]);
+      const int at = (j * 16 + 4 * h) * (int)sizeof(T);
+      *(Pack<T, 4> *)(mine + place(i * 16 + c, at / 16) + at % 16) = out;
+    }
+  }
+  // (a wave reads what it wrote itself)
+  const int per_store = 64 / CHUNKS; // rows
+  const bool whole = whole_pieces<T>(p, 16 / (int)sizeof(T));
+#pragma unroll 4
+  for (int r0 = 0; r0 < TM * 16; r0 += per_store) {
+    const int row = r0 + lane / CHUNKS, q = lane % CHUNKS;
+    const int m = m0 + wm * (TM * 16) + row;
+    const int n = n0 + wn * (TN * 16) + q * (16 / (int)sizeof(T));
+    if (lane >= per_store * CHUNKS || row >= TM * 16 || m >= p.M || n >= p.N)
+      continue;
+    const v4u w = *(const v4u *)(mine + place(row, q));
+    T *const y = (T *)p.y + (int64_t)m * p.N + n;
+    if (whole) {
+      *(v4u *)y = w;
+    } else {
+      const Pack<T, 16 / sizeof(T)> e = __builtin_bit_cast(Pack<T, 16 / sizeof(T)>, w);
+#pragma unroll
+      for (int i = 0; i < 16 / (int)sizeof(T); ++i)
+        if (n + i < p.N)
+          y[i] = e.v[i];
+    }
+  }
+}
+
+// The parts' sums added in their order, four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void k_join_parts(const GemmParams p) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const unsigned quads = (unsigned)p.part_pitch / 4;
+  const int64_t m = id / quads;
+  const int n = (int)(id - m * quads) * 4;
+  if (m >= p.M)
+    return;
+  v4f t = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = 0; i < p.parts; ++i)
+    t += *(const v4f *)(p.part_sums + ((int64_t)i * p.M + m) * p.part_pitch + n);
+  const float v[4] = {t[0], t[1], t[2], t[3]};
+  store4<T>(p, (int)m, n, v);
 }
 
 // Rows copied to a pitch of whole 16-byte chunks, zeros behind them.
@@ -624,6 +767,7 @@ hipError_t skinny(hipStream_t st, const GemmParams &p) {
   const dim3 grid((unsigned)((p.N + 15) / 16));
   const bool tail = p.K % kBlock != 0 || !rows_aligned(p.a, p.lda) || !rows_aligned(p.b, p.ldb);
   constexpr int D = MT > 2 ? 2 : 4;
+  note_gemm_kernel("k_block_skinny");
   if (tail)
     k_block_skinny<T, MT, 4, 2, true><<<grid, 256, 0, st>>>(p);
   else if (grid.x <= 512 && p.kblocks >= 16)
@@ -633,31 +777,116 @@ hipError_t skinny(hipStream_t st, const GemmParams &p) {
   return hipGetLastError();
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+// Tiles that a product can be dealt in.
+enum TileForm { k256x256, k256x128, k128x128, k64x128, kTileForms };
+
+// Which tile, and in how many parts of K: what takes the least time by
+//   base + steps (full rounds * full + the rest of the fullest CU * lone) + rounds * round
+//   [+ 3.7 + 1.43 us per million sums of all parts, to write, read and add them]
+// microseconds, where a CU holds per_cu tiles at once and takes its share of them
+// one round after the other.  Fitted to 872 products of 80 .. 4096 rows timed in
+// every form (relative errors 6 - 10 %); the forms that it takes are 1.4 % slower
+// than the fastest in the geometric mean, 14 % at most.
+struct TileCost {
+  int bm, bn, per_cu;
+  float base, full, lone, round;
+};
+constexpr TileCost kTileCosts16[kTileForms] = {
+    {256, 256, 1, 3.2f, 0.0f, 1.54f, 1.83f},
+    {256, 128, 1, 4.7f, 0.0f, 0.91f, 0.0f},
+    {128, 128, 2, 3.7f, 1.08f, 0.74f, 0.0f},
+    {64, 128, 2, 2.7f, 0.77f, 0.59f, 0.0f},
+};
+constexpr TileCost kTileCosts32[kTileForms] = { // (the first two are not there)
+    {0, 0, 0, 0, 0, 0, 0},
+    {0, 0, 0, 0, 0, 0, 0},
+    {128, 128, 2, 5.1f, 1.76f, 1.04f, 0.0f},
+    {64, 128, 2, 3.4f, 1.12f, 0.76f, 0.0f},
+};
+struct TilePlan {
+  int form, parts;
+};
+constexpr int kMostParts = 16;
+constexpr int64_t kMostSums = (int64_t)64 << 20; // of all parts
+TilePlan plan_tiles(const BlockGemm &g) {
+  const int64_t kblocks = (g.K + kBlock - 1) / kBlock;
+  TilePlan best = {k128x128, 1};
+  float least = 0.0f;
+  for (int form = 0; form < kTileForms; ++form) {
+    const TileCost &c = g.kind == kF32 ? kTileCosts32[form] : kTileCosts16[form];
+    if (!c.bm)
+      continue;
+    const int64_t tiles = ((g.M + c.bm - 1) / c.bm) * ((g.N + c.bn - 1) / c.bn);
+    for (int parts = 1; parts <= kMostParts; parts *= 2) {
+      if (parts > 1 && (parts > kblocks || g.M * g.N > kMostSums / parts))
+        break;
+      const int64_t steps = (kblocks + parts - 1) / parts;
+      const int64_t n = (tiles * parts + 255) / 256; // on the fullest CU
+      const int64_t full = n / c.per_cu, rest = n % c.per_cu;
+      // (one tile at a time: every round is a lone one)
+      float us = c.base + c.round * (float)(full + (rest > 0));
+      us += (float)steps * (c.per_cu > 1 ? full * c.full + rest * c.lone : full * c.lone);
+      if (parts > 1)
+        us += 3.7f + 1.43e-6f * (float)(parts * g.M * g.N);
+      if (least == 0.0f || us < least) {
+        least = us;
+        best = {form, parts};
+      }
+    }
+  }
+  return best;
+}
+
+const char *tile_name(int bm, int bn, bool parts) {
+  if (bm == 256)
+    return bn == 256 ? (parts ? "k_block_tile (256x256, K in parts)" : "k_block_tile (256x256)")
+                     : (parts ? "k_block_tile (256x128, K in parts)" : "k_block_tile (256x128)");
+  return bm == 128 ? (parts ? "k_block_tile (128x128, K in parts)" : "k_block_tile (128x128)")
+                   : (parts ? "k_block_tile (64x128, K in parts)" : "k_block_tile (64x128)");
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 hipError_t tile(hipStream_t st, const GemmParams &p) {
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int kLds = 2 * (BM + BN) * kBlock;
-  auto *const kernel = k_block_tile<T, BM, BN, WM, WN, kExact>;
+  constexpr int kLds = STAGES * (BM + BN) * kBlock + 2 * WM * WN * 1024;
+  static_assert(kLds <= 160 * 1024, "LDS");
+  auto *const kernel = k_block_tile<T, BM, BN, WM, WN, STAGES, kExact>;
   if (kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void *)kernel,
         hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess)
       return e;
   }
+  note_gemm_kernel(tile_name(BM, BN, p.parts > 1));
   const unsigned tiles = (unsigned)((p.M + BM - 1) / BM) * (unsigned)((p.N + BN - 1) / BN);
-  kernel<<<dim3(tiles), WM * WN * 64, kLds, st>>>(p);
-  return hipGetLastError();
+  kernel<<<dim3(tiles * p.parts), WM * WN * 64, kLds, st>>>(p);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.parts > 1) {
+    const int64_t n = (int64_t)p.M * (p.part_pitch / 4);
+    k_join_parts<T><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(p);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 template <typename T>
-hipError_t product(hipStream_t st, const GemmParams &p) {
+hipError_t product(hipStream_t st, const GemmParams &p, int form) {
   if (p.M <= 16)
     return skinny<T, 1>(st, p);
   if (p.M <= 32)
     return skinny<T, 2>(st, p);
   if (p.M <= kSkinnyRows)
     return skinny<T, 4>(st, p);
-  return tile<T, 128, 128, 2, 2>(st, p);
+  // (f32 results of larger tiles do not fit in LDS)
+  if constexpr (sizeof(T) == 2) {
+    switch (form) {
+    case k256x256:
+      return tile<T, 256, 256, 2, 4, 2>(st, p);
+    case k256x128:
+      return tile<T, 256, 128, 4, 2, 3>(st, p);
+    }
+  }
+  return form == k64x128 ? tile<T, 64, 128, 1, 4, 2>(st, p) : tile<T, 128, 128, 2, 2, 2>(st, p);
 }
 
 } // namespace
@@ -682,10 +911,14 @@ hipError_t launch_quantize_blocks(hipStream_t s, const void *x, FloatKind kind,
 static size_t aligned_bytes(const void *p, int64_t rows, int64_t K) {
   return rows_aligned(p, K) ? 0 : (size_t)rows * (size_t)((K + 15) / 16 * 16);
 }
+static int64_t part_pitch(const BlockGemm &g) { return (g.N + 3) / 4 * 4; }
+static size_t parts_bytes(const BlockGemm &g, const TilePlan &plan) {
+  return plan.parts > 1 ? (size_t)plan.parts * g.M * part_pitch(g) * sizeof(float) : 0;
+}
 size_t block_gemm_scratch(const BlockGemm &g) {
   if (g.M <= kSkinnyRows)
     return 0;
-  return aligned_bytes(g.a, g.M, g.K) + aligned_bytes(g.b, g.N, g.K);
+  return aligned_bytes(g.a, g.M, g.K) + aligned_bytes(g.b, g.N, g.K) + parts_bytes(g, plan_tiles(g));
 }
 
 hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
@@ -702,9 +935,18 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
   p.kblocks = (int)((g.K + kBlock - 1) / kBlock);
   p.bias_step = g.bias_len > 1;
   p.activation = g.activation;
+  p.parts = 1;
+  p.part_blocks = p.kblocks;
+  TilePlan plan = {};
   if (g.M > kSkinnyRows) {
-    const int pitch = (int)((g.K + 15) / 16 * 16);
+    plan = plan_tiles(g);
     uint8_t *at = (uint8_t *)scratch;
+    p.parts = plan.parts;
+    p.part_blocks = (p.kblocks + plan.parts - 1) / plan.parts;
+    p.part_pitch = (int)part_pitch(g);
+    p.part_sums = (float *)at;
+    at += parts_bytes(g, plan); // (a multiple of 16)
+    const int pitch = (int)((g.K + 15) / 16 * 16);
     auto align = [&](const uint8_t *&rows_of, int64_t rows, int &ld) {
       if (rows_aligned(rows_of, g.K))
         return hipSuccess;
@@ -726,11 +968,11 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
   }
   switch (g.kind) {
   case kF32:
-    return product<float>(s, p);
+    return product<float>(s, p, plan.form);
   case kF16:
-    return product<_Float16>(s, p);
+    return product<_Float16>(s, p, plan.form);
   default:
-    return product<__bf16>(s, p);
+    return product<__bf16>(s, p, plan.form);
   }
 }
 

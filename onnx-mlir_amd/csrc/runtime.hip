@@ -2567,8 +2567,9 @@ void om_mi355x_MatMulBlocks(OMTensor *y_t, const OMTensor *a_t,
   bool relu, gelu;
   if (!activation_ok(activation, op, relu, gelu))
     return;
-  if (g.M > kMostOfOne || g.N > kMostOfOne || g.K > kMostOfOne ||
-      blocks_of(g.M) * blocks_of(g.N) > kMostBlocks) {
+  // (rows of a tile are addressed by 31-bit offsets)
+  if (g.M > kMostOfOne || g.N > kMostOfOne || g.K > ((int64_t)1 << 22) ||
+      blocks_of(g.M) * blocks_of(g.N) > kMostBlocks / 32) {
     fail(EINVAL, "%s: the product is too large", op);
     return;
   }

@@ -158,6 +158,12 @@ def check_product(om, got, want, size, dtype, rows, K):
     # Gelu: its slope is below 1.13, its own error below 2^-21 of its argument
     off = (128 + -(-K // 128) + 16) * 2.0 ** -24 + (2.0 ** -12 if dtype != "f32" and rows > 64 else 0)
     limit = size * (1.13 * off + 2.0 ** -21) + ref.half_step(dtype) * np.abs(want) * (1 + 2.0 ** -8) + ref.smallest_step(dtype)
+    if dtype == "f16":  # 65520 and more round to infinity
+        over = np.abs(want) - limit >= 65520
+        assert np.array_equal(got[over], np.copysign(np.inf, want[over]))
+        near = ~over & (np.abs(want) + limit < 65520)
+        assert np.isfinite(got[near]).all()
+        got, want, limit = got[near], want[near], limit[near]
     assert np.all(np.abs(got - want) <= limit), (np.abs(got - want) / limit).max()
 
 
@@ -171,6 +177,36 @@ def test_matmul_blocks(om, M, K, N, dtype):
     got = om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), on(om, sb), dtype=dt(om, dtype))
     want, size = product(om, a, sa, b, sb)
     check_product(om, back(om, got), want, size, dtype, M, K)
+
+
+@pytest.mark.parametrize("M,K,N,dtype,kernel", [
+    (40, 4096, 300, "bf16", "k_block_skinny"),
+    (130, 768, 768, "f16", "k_block_tile (64x128)"),
+    (2048, 384, 4096, "bf16", "k_block_tile (128x128)"),
+    (512, 1040, 11008, "bf16", "k_block_tile (256x128)"),
+    (4000, 1024, 4096, "f16", "k_block_tile (256x256)"),
+    (80, 4096, 4090, "bf16", "k_block_tile (64x128, K in parts)"),
+    (90, 4208, 11008, "f16", "k_block_tile (64x128)"),
+    (65, 4096, 11008, "f16", "k_block_tile (128x128, K in parts)"),
+    (700, 11008, 1024, "bf16", "k_block_tile (256x128, K in parts)"),
+    (100, 4176, 1024, "f32", "k_block_tile (64x128, K in parts)"),
+    (2048, 2048, 4096, "f32", "k_block_tile (128x128)")])
+def test_matmul_blocks_in_every_form(om, M, K, N, dtype, kernel):
+    rng = np.random.default_rng(M + K + N)
+    a, b = (rng.integers(0, 256, s, dtype=np.uint8) for s in ((M, K), (N, K)))
+    for x in (a, b):
+        x[(x & 127) == 127] = 0x40  # no NaN
+    kb = -(-K // 128)
+    sa, sb = (rng.uniform(0.5, 2, s).astype(np.float32) for s in ((M, kb), (-(-N // 128), kb)))
+    a, b = a.view(om.float8_e4m3fn), b.view(om.float8_e4m3fn)
+    c = rng.standard_normal(N).astype(np.float32)
+    args = [on(om, t) for t in (a, sa, b, sb, c)]
+    got = om.MatMulBlocks(*args, dtype=dt(om, dtype))
+    assert om.last_gemm_kernel() == kernel
+    want, size = product(om, a, sa, b, sb, c)
+    check_product(om, back(om, got), want, size, dtype, M, K)
+    again = om.MatMulBlocks(*args, dtype=dt(om, dtype))
+    assert np.array_equal(bits(again.numpy()), bits(got.numpy()))
 
 
 @pytest.mark.parametrize("act", [0, 1, 2])
