@@ -220,7 +220,7 @@ hipError_t quantize(hipStream_t st, const T *x, int64_t M, int64_t K, int rows,
 // below that of f16 (2.1e-4), and they run twice as fast as those for bf16, so
 // results in 16 bits take them.  Results in f32 are summed by the bf16
 // instructions (6e-8 to 1.4e-7 on the same operands), which hold every e4m3
-// value exactly; so does everything that is bound by reading its weights.
+// value exactly; so are those of few rows, which are bound by reading weights.
 
 // Four e4m3 values of a word, two to each result.
 __device__ __forceinline__ void widen4(unsigned w, v2bf &lo, v2bf &hi) {
@@ -277,11 +277,13 @@ __device__ __forceinline__ float finish(float v, const GemmParams &p, float bias
   return v;
 }
 
-// Whether rows of y divide into aligned pieces of n elements.
-template <typename T>
-__device__ __forceinline__ bool whole_pieces(const GemmParams &p, int n) {
-  return p.N % n == 0 && (uintptr_t)p.y % (n * sizeof(T)) == 0;
-}
+// 16 bytes at any element of type T.
+template <typename T> struct Loose {
+  typedef unsigned v4 __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct Loose<float> {
+  typedef unsigned v4 __attribute__((ext_vector_type(4), aligned(4)));
+};
 
 // Four neighbouring columns n .. n + 3 of row m; those past N are left out.
 template <typename T>
@@ -295,8 +297,11 @@ __device__ __forceinline__ void store4(
     const float bias = p.bias ? p.bias[c * p.bias_step] : 0.0f;
     t[i] = from_f32<T>(finish(v[i], p, bias));
   }
-  if (whole_pieces<T>(p, 4) && n + 4 <= p.N) {
-    *(Pack<T, 4> *)y = *(const Pack<T, 4> *)t;
+  if (n + 4 <= p.N) { // (rows may start at any element)
+    struct __attribute__((packed, aligned(alignof(T)))) Four {
+      T v[4];
+    };
+    *(Four *)y = Four{{t[0], t[1], t[2], t[3]}};
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -305,15 +310,31 @@ __device__ __forceinline__ void store4(
   }
 }
 
+// 16 bytes a lane from `from` + at + k (k the same in all lanes; nothing from
+// `bytes` on) into LDS, the wave's from `to` on, one after the other.
+__device__ __forceinline__ void copy16(
+    const void *from, void *to, int at, int k, unsigned bytes = 0x7FFFFFFF) {
+  typedef __attribute__((address_space(3))) void *lds_ptr;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(
+      __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, bytes, 0x00020000),
+      (lds_ptr)to, 16, at, k, 0, 0);
+}
+
 // --- few rows ---------------------------------------------------------------
 // Up to 16 MT rows: a block owns 16 columns, its WAVES waves take every
-// WAVES-th block of 128 of K.  Bound by reading the weights once: a wave has
-// the weights of DEPTH blocks on their way, lanes (c, h) the bytes 16 h .. of
-// each half of column c's 128, whole lines together.  Products by bf16
+// WAVES-th block of 128 of K.  Bound by reading the weights once: a wave has the
+// weights of DEPTH blocks on their way, lanes (c, h) the bytes 16 h .. of each half
+// of column c's 128, whole lines together; rows of a that are not there are not
+// asked for.  Scales come by way of LDS, once a block: asked for by every wave,
+// the few lines that hold them are what L2 is busiest with.  Products by bf16
 // instructions; sums of the waves meet in LDS in a fixed order.
-template <typename T, int MT, int WAVES, int DEPTH, bool TAIL>
+// One row, 4096 x 11008: 11.5 us (12.4 with scales asked for by every wave, 11.9
+// with the weights copied into LDS, 9.8 with neither rows of a nor scales).
+// TAIL: any K and any alignment, what lies past a row's end 0.
+template <typename T, int MT, int WAVES, int DEPTH, bool TAIL, bool STAGED>
 __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p) {
-  __shared__ float sums[WAVES][MT][64][4];
+  extern __shared__ float staged[]; // scales of b's columns, then of a's rows
+  __shared__ v4f sums[WAVES][MT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, h = lane >> 4;
@@ -321,12 +342,11 @@ __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p)
   const int col = n0 + c < p.N ? n0 + c : p.N - 1;
   const uint8_t *const b = p.b + (int64_t)col * p.ldb + 16 * h;
   const uint8_t *a[MT];
-  const float *as[MT];
+  int a_row[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int row = 16 * i + c < p.M ? 16 * i + c : p.M - 1;
-    a[i] = p.a + (int64_t)row * p.lda + 16 * h;
-    as[i] = p.a_scale + (int64_t)row * p.kblocks;
+    a_row[i] = 16 * i + c < p.M ? 16 * i + c : p.M - 1;
+    a[i] = p.a + (int64_t)a_row[i] * p.lda + 16 * h;
   }
   const float *const bs = p.b_scale + (int64_t)(n0 / kBlock) * p.kblocks;
 
@@ -338,7 +358,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p)
       total[i][r] = 0.0f;
 
   v4u wb[DEPTH][2], wa[DEPTH][MT][2];
-  float sa[DEPTH][MT], sb[DEPTH];
   // 16 bytes of a row from k on; past its end they are 0.
   auto load16 = [&](const uint8_t *row, int k) -> v4u {
     if (!TAIL)
@@ -361,24 +380,47 @@ __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p)
     for (int half = 0; half < 2; ++half) {
       wb[d][half] = load16(b, k + 64 * half);
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-        wa[d][i][half] = load16(a[i], k + 64 * half);
+      for (int i = 0; i < MT; ++i) {
+        wa[d][i][half] = v4u{0, 0, 0, 0};
+        if (16 * i + c < p.M)
+          wa[d][i][half] = load16(a[i], k + 64 * half);
+      }
     }
-    sb[d] = bs[kb];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      sa[d][i] = as[i][kb];
   };
+  // (the scales are asked for first: loads come back in order)
+  const int scales = (p.M + 1) * p.kblocks;
+  auto scale = [&](int i) {
+    i = i < scales ? i : scales - 1;
+    return i < p.kblocks ? bs + i : p.a_scale + (i - p.kblocks);
+  };
+  float mine = 0.0f;
+  if (STAGED && scales > 0)
+    mine = *scale(threadIdx.x);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
     if (wave + d * WAVES < p.kblocks)
       fetch(d, wave + d * WAVES);
+  if (STAGED) {
+    __builtin_amdgcn_sched_barrier(0);
+    if ((int)threadIdx.x < scales)
+      staged[threadIdx.x] = mine;
+    for (int i = threadIdx.x + WAVES * 64; i < scales; i += WAVES * 64)
+      staged[i] = *scale(i);
+    gemm::lds_barrier();
+  }
+  auto b_scale = [&](int kb) { return STAGED ? staged[kb] : bs[kb]; };
+  auto a_scale = [&](int i, int kb) {
+    return STAGED ? staged[p.kblocks + a_row[i] * p.kblocks + kb]
+                  : p.a_scale[(int64_t)a_row[i] * p.kblocks + kb];
+  };
   for (int kb = wave; kb < p.kblocks; kb += DEPTH * WAVES) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int at = kb + d * WAVES;
       if (at >= p.kblocks)
         break;
+      const float sb = b_scale(at);
       v4f acc[MT];
 #pragma unroll
       for (int i = 0; i < MT; ++i)
@@ -395,40 +437,26 @@ __global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p)
                 0, 0);
         }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const float s = sa[d][i] * sb[d];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          total[i][r] = __builtin_fmaf(acc[i][r], s, total[i][r]);
-      }
+      for (int i = 0; i < MT; ++i)
+        add_scaled(total[i], acc[i], a_scale(i, at) * sb);
       if (at + DEPTH * WAVES < p.kblocks)
         fetch(d, at + DEPTH * WAVES);
     }
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
-    *(v4f *)sums[wave][i][lane] = v4f{total[i][0], total[i][1], total[i][2], total[i][3]};
+    sums[wave][i][lane] = v4f{total[i][0], total[i][1], total[i][2], total[i][3]};
   __syncthreads();
   // lane (c, h) of wave i: row 16 i + c, columns n0 + 4 h ..
   for (int i = wave; i < MT; i += WAVES) {
     v4f t = {0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < WAVES; ++w)
-      t += *(const v4f *)sums[w][i][lane];
+      t += sums[w][i][lane];
     const float v[4] = {t[0], t[1], t[2], t[3]};
     if (16 * i + c < p.M)
       store4<T>(p, 16 * i + c, n0 + 4 * h, v);
   }
-}
-
-// 16 bytes a lane from `from` + at + k (k the same in all lanes; nothing from
-// `bytes` on) into LDS, the wave's from `to` on, one after the other.
-__device__ __forceinline__ void copy16(
-    const void *from, void *to, int at, int k, unsigned bytes = 0x7FFFFFFF) {
-  typedef __attribute__((address_space(3))) void *lds_ptr;
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(
-      __builtin_amdgcn_make_buffer_rsrc((void *)from, 0, bytes, 0x00020000),
-      (lds_ptr)to, 16, at, k, 0, 0);
 }
 
 // --- tiles ------------------------------------------------------------------
@@ -694,7 +722,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams
   }
   // (a wave reads what it wrote itself)
   const int per_store = 64 / CHUNKS; // rows
-  const bool whole = whole_pieces<T>(p, 16 / (int)sizeof(T));
+  // (rows may start at any element: stores of 16 bytes need no more than theirs)
+  typedef typename Loose<T>::v4 v4u_any;
 #pragma unroll 4
   for (int r0 = 0; r0 < TM * 16; r0 += per_store) {
     const int row = r0 + lane / CHUNKS, q = lane % CHUNKS;
@@ -704,8 +733,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams
       continue;
     const v4u w = *(const v4u *)(mine + place(row, q));
     T *const y = (T *)p.y + (int64_t)m * p.N + n;
-    if (whole) {
-      *(v4u *)y = w;
+    if (n + 16 / (int)sizeof(T) <= p.N) {
+      *(v4u_any *)y = w;
     } else {
       const Pack<T, 16 / sizeof(T)> e = __builtin_bit_cast(Pack<T, 16 / sizeof(T)>, w);
 #pragma unroll
@@ -733,48 +762,67 @@ __global__ __launch_bounds__(256) void k_join_parts(const GemmParams p) {
   store4<T>(p, (int)m, n, v);
 }
 
-// Rows copied to a pitch of whole 16-byte chunks, zeros behind them.
-__global__ __launch_bounds__(256) void k_align_rows(
-    const uint8_t *from, uint8_t *to, int64_t rows, int K, int pitch) {
+// Rows of up to two matrices copied to a pitch of whole 16-byte chunks, zeros
+// behind them.
+struct AlignRows {
+  const uint8_t *from[2];
+  uint8_t *to[2];
+  int64_t rows[2];
+  int K, pitch;
+};
+__global__ __launch_bounds__(256) void k_align_rows(const AlignRows p) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int chunks = pitch / 16;
-  const int64_t row = id / chunks;
+  const int chunks = p.pitch / 16;
+  int64_t row = id / chunks;
   const int k = (int)(id - row * chunks) * 16;
-  if (row >= rows)
+  const int which = row >= p.rows[0];
+  row -= which ? p.rows[0] : 0;
+  if (row >= p.rows[which])
     return;
-  const uint8_t *const x = from + row * K + k;
+  const uint8_t *const x = p.from[which] + row * p.K + k;
   v4u w = {0, 0, 0, 0};
-  if (k + 16 <= K) {
+  if (k + 16 <= p.K) {
     typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
     w = *(const v4u_any *)x;
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (k + i < K)
+      if (k + i < p.K)
         w[i / 4] |= (unsigned)x[i] << (8 * (i % 4));
   }
-  *(v4u *)(to + row * pitch + k) = w;
+  *(v4u *)(p.to[which] + row * p.pitch + k) = w;
 }
 
-constexpr int kSkinnyRows = 64;
+// Rows that the kernel for few of them takes: 16, and 32 of small products, where a
+// tile's steps cost more than fetching a's rows in every block (32 rows, skinny /
+// tiles: 768x768 4.5 / 5.5, 2048x2048 7.5 / 7.5, 4096x1024 9.2 / 8.3, 4096x11008
+// 26 / 14 us).
+bool few_rows(int64_t M, int64_t K, int64_t N) {
+  return M <= 16 || (M <= 32 && K * N < (int64_t)1 << 21);
+}
 
 bool rows_aligned(const void *p, int64_t K) {
   return K % 16 == 0 && ((uintptr_t)p & 15) == 0;
 }
 
+template <typename T, int MT, int WAVES, int DEPTH, bool TAIL>
+hipError_t skinny_in(hipStream_t st, const GemmParams &p) {
+  const dim3 grid((unsigned)((p.N + 15) / 16)), block(WAVES * 64);
+  // (32 KB of scales: 16 rows of 61000 elements)
+  const int64_t floats = (int64_t)(p.M + 1) * p.kblocks;
+  if (floats <= 8192)
+    k_block_skinny<T, MT, WAVES, DEPTH, TAIL, true><<<grid, block, (size_t)floats * 4, st>>>(p);
+  else
+    k_block_skinny<T, MT, WAVES, DEPTH, TAIL, false><<<grid, block, 0, st>>>(p);
+  return hipGetLastError();
+}
+
 template <typename T, int MT>
 hipError_t skinny(hipStream_t st, const GemmParams &p) {
-  const dim3 grid((unsigned)((p.N + 15) / 16));
-  const bool tail = p.K % kBlock != 0 || !rows_aligned(p.a, p.lda) || !rows_aligned(p.b, p.ldb);
-  constexpr int D = MT > 2 ? 2 : 4;
   note_gemm_kernel("k_block_skinny");
-  if (tail)
-    k_block_skinny<T, MT, 4, 2, true><<<grid, 256, 0, st>>>(p);
-  else if (grid.x <= 512 && p.kblocks >= 16)
-    k_block_skinny<T, MT, 8, D, false><<<grid, 512, 0, st>>>(p);
-  else
-    k_block_skinny<T, MT, 4, D, false><<<grid, 256, 0, st>>>(p);
-  return hipGetLastError();
+  if (p.K % kBlock != 0 || !rows_aligned(p.a, p.lda) || !rows_aligned(p.b, p.ldb))
+    return skinny_in<T, MT, 8, 2, true>(st, p);
+  return skinny_in<T, MT, (MT > 1 ? 4 : 8), 4, false>(st, p);
 }
 
 // Tiles that a product can be dealt in.
@@ -871,12 +919,8 @@ hipError_t tile(hipStream_t st, const GemmParams &p) {
 
 template <typename T>
 hipError_t product(hipStream_t st, const GemmParams &p, int form) {
-  if (p.M <= 16)
-    return skinny<T, 1>(st, p);
-  if (p.M <= 32)
-    return skinny<T, 2>(st, p);
-  if (p.M <= kSkinnyRows)
-    return skinny<T, 4>(st, p);
+  if (few_rows(p.M, p.K, p.N))
+    return p.M <= 16 ? skinny<T, 1>(st, p) : skinny<T, 2>(st, p);
   // (f32 results of larger tiles do not fit in LDS)
   if constexpr (sizeof(T) == 2) {
     switch (form) {
@@ -916,7 +960,7 @@ static size_t parts_bytes(const BlockGemm &g, const TilePlan &plan) {
   return plan.parts > 1 ? (size_t)plan.parts * g.M * part_pitch(g) * sizeof(float) : 0;
 }
 size_t block_gemm_scratch(const BlockGemm &g) {
-  if (g.M <= kSkinnyRows)
+  if (few_rows(g.M, g.K, g.N))
     return 0;
   return aligned_bytes(g.a, g.M, g.K) + aligned_bytes(g.b, g.N, g.K) + parts_bytes(g, plan_tiles(g));
 }
@@ -938,7 +982,7 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
   p.parts = 1;
   p.part_blocks = p.kblocks;
   TilePlan plan = {};
-  if (g.M > kSkinnyRows) {
+  if (!few_rows(g.M, g.K, g.N)) {
     plan = plan_tiles(g);
     uint8_t *at = (uint8_t *)scratch;
     p.parts = plan.parts;
@@ -947,22 +991,29 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
     p.part_sums = (float *)at;
     at += parts_bytes(g, plan); // (a multiple of 16)
     const int pitch = (int)((g.K + 15) / 16 * 16);
+    AlignRows copies = {};
+    int n = 0;
     auto align = [&](const uint8_t *&rows_of, int64_t rows, int &ld) {
       if (rows_aligned(rows_of, g.K))
-        return hipSuccess;
-      const int64_t n = rows * (pitch / 16);
-      k_align_rows<<<dim3((unsigned)((n + 255) / 256)), 256, 0, s>>>(
-          rows_of, at, rows, (int)g.K, pitch);
+        return;
+      copies.from[n] = rows_of;
+      copies.to[n] = at;
+      copies.rows[n++] = rows;
       rows_of = at;
       ld = pitch;
       at += (size_t)rows * pitch;
-      return hipGetLastError();
     };
-    hipError_t e = align(p.a, g.M, p.lda);
-    if (e == hipSuccess)
-      e = align(p.b, g.N, p.ldb);
-    if (e != hipSuccess)
-      return e;
+    align(p.a, g.M, p.lda);
+    align(p.b, g.N, p.ldb);
+    if (n) {
+      copies.K = (int)g.K;
+      copies.pitch = pitch;
+      const int64_t chunks = (copies.rows[0] + copies.rows[1]) * (pitch / 16);
+      k_align_rows<<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>(copies);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess)
+        return e;
+    }
     if (p.lda == pitch && p.ldb == pitch)
       p.K = pitch; // (zeros behind the last element of both)
   }
