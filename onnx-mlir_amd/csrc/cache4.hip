@@ -11,6 +11,7 @@
 
 #include <type_traits>
 
+#include "gemm_common.h"
 #include "llm_common.h"
 
 namespace om {
@@ -694,6 +695,524 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
   }
 }
 
+// ---------------------------------------------------------------------------
+// attention of many rows
+// ---------------------------------------------------------------------------
+// Where a head of keys has many rows, and their type 16 bits, what bounds the
+// kernel above is scaling and splitting weights anew in every wave.  Here a block
+// of 128 rows makes 64 keys and values at a time into f16 in LDS, s c + m with one
+// rounding (2^-11; what lies beyond 65504, up to which rows are stored, becomes
+// that), and its waves multiply those by q, which f16 holds (bf16 ones with each
+// row's largest at 2^14, so that what f16 drops of others is 2^-38 of it), and by p
+// in f16 (2^-11 again), 2^7 times what it is relative to a maximum that is at most 8
+// powers of two behind: what f16 loses of p is below 2^-32 of the largest.  Sums,
+// scores and statistics are f32.
+//
+// A wave has 32 rows in two tiles: both operands that it reads from LDS, 1 KB each,
+// feed two instructions, which is as fast as LDS can feed four waves.  Scores'
+// layout is that of the second product's operand, as above.
+//
+// LDS: keys' fragments (u, f), u of four 16s, f of G: lane (c, h) has word f of the
+// quarter h of key c's codes, 8 elements; values' (half, t): lane (c, h) has, of the
+// keys 4 h .. of either 16, element 16 t + c in the order z (4 G) + j: byte z / 2 of
+// word j, z % 2 its half.  All are read as they lie, 1024 bytes after one another.
+//
+// A group of a value whose scale or lowest value is not finite must give NaN to rows
+// that see its key and nothing to others: it is made into zeros, and marked.
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+constexpr unsigned kUnknown = 1u << 31; // a key without a place in the cache
+constexpr int kPromptRows = 128;
+
+__device__ __forceinline__ v2h halves_of(unsigned w) { return __builtin_bit_cast(v2h, w); }
+__device__ __forceinline__ unsigned low_halves(unsigned a, unsigned b) {
+  return __builtin_amdgcn_perm(b, a, 0x05040100);
+}
+__device__ __forceinline__ unsigned high_halves(unsigned a, unsigned b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302);
+}
+// Codes in bits 0 .. 3 (LOW) or 4 .. 7 of the halves of w, as f16: 1024 + code
+// and 1024 + 16 code have the bits 0x6400 | code.
+template <bool LOW> __device__ __forceinline__ v2h codes_of(unsigned w) {
+  if (LOW)
+    return halves_of((w & 0x000F000Fu) | 0x64006400u) - v2h{1024, 1024};
+  return __builtin_elementwise_fma(halves_of((w & 0x00F000F0u) | 0x64006400u),
+      v2h{0.0625f16, 0.0625f16}, v2h{-64, -64});
+}
+__device__ __forceinline__ v2h within(v2h x) { // NaN stays
+  const _Float16 top = 65504;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    x[i] = x[i] > top ? top : x[i] < -top ? -top : x[i];
+  return x;
+}
+__device__ __forceinline__ bool is_finite(_Float16 x) {
+  return (__builtin_bit_cast(unsigned short, x) & 0x7C00) != 0x7C00;
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Arguments p) {
+  constexpr int D = 32 * G, WORDS = 4 * G, ITEMS = (WORDS + 15) / 16;
+  constexpr int SG = G < 4 ? G : 4; // groups of a word's bytes
+  constexpr int PITCH = 2 * D + 16; // of a row of results in LDS
+  extern __shared__ __attribute__((aligned(16))) float shared[];
+  uint8_t *const keys = (uint8_t *)shared, *const values = keys + G * 4096;
+  // [parity][key]: groups of its value that are not finite, and whether it is known
+  unsigned *const marks = (unsigned *)(values + G * 4096);
+  const int lane = threadIdx.x & 63, c = lane & 15, h = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float inf = __builtin_inff();
+
+  const int id = xcd_contiguous(blockIdx.x, (int)gridDim.x);
+  const int split = (unsigned)id % (unsigned)p.splits;
+  const int unit = (unsigned)id / (unsigned)p.splits;
+  const int bh = (unsigned)unit / (unsigned)p.groups;
+  int group = unit - bh * p.groups;
+  const int b = (unsigned)bh / (unsigned)p.c.H, head = (unsigned)bh % (unsigned)p.c.H;
+  if (p.causal) // those with the most keys first
+    group = p.groups - 1 - group;
+
+  const int past = p.c.past[b];
+  int count = p.S;
+  if (p.c.counts) {
+    const int n = p.c.counts[b];
+    count = n < 0 ? 0 : n < p.S ? n : p.S;
+  }
+  const int rows = count * p.per_head, row0 = group * kPromptRows;
+  if (row0 >= rows)
+    return;
+  const int last_row = (row0 + kPromptRows < rows ? row0 + kPromptRows : rows) - 1;
+  const unsigned page_size = (unsigned)p.c.page_size;
+  const int capacity = (int)(p.c.table ? p.c.table_pages * p.c.page_size : p.c.page_size);
+  // Keys [first, end) of the query of token i.
+  const int start = p.starts ? p.starts[b] : 0;
+  auto first_of = [&](int i) -> int {
+    int64_t f = start > 0 ? start : 0;
+    if (p.window > 0 && past + (int64_t)i - p.window + 1 > f)
+      f = past + (int64_t)i - p.window + 1;
+    return (int)(f < capacity ? f : capacity);
+  };
+  auto end_of = [&](int i) -> int {
+    const int64_t e = past + (int64_t)(p.causal ? i : count - 1) + 1;
+    return (int)(e < 0 ? 0 : e < capacity ? e : capacity);
+  };
+  int tile, tiles; // of 64 keys: this part's
+  {
+    const int lo = first_of(row0 / p.per_head), hi = end_of(last_row / p.per_head);
+    tile = lo / 64;
+    tiles = hi > lo ? (hi + 63) / 64 - tile : 0;
+    const int each = (tiles + p.splits - 1) / p.splits;
+    tile += split * each;
+    tiles = tiles - split * each < each ? tiles - split * each : each;
+  }
+  // Keys that some, and that all of the wave's rows see.
+  int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
+  if (row0 + 32 * wave < rows) {
+    const int r1 = row0 + 32 * wave + 31;
+    const int i0 = (row0 + 32 * wave) / p.per_head, i1 = (r1 < rows ? r1 : rows - 1) / p.per_head;
+    lo = first_of(i0), hi = end_of(i1);
+    all_lo = first_of(i1), all_hi = end_of(i0);
+  }
+
+  // This lane's rows: q in the order of a word's codes as they come out of it.
+  const float scale =
+      (p.scale ? p.scale[0] : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
+  v8h q[2][G];
+  float by[2]; // a score's factor
+  int row_lo[2], row_hi[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    int row = row0 + 32 * wave + 16 * r + c;
+    row = row < rows ? row : rows - 1;
+    const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
+    row_lo[r] = first_of(i);
+    row_hi[r] = end_of(i);
+    const int64_t at = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
+                                     : ((int64_t)b * p.S + i) * p.heads + qh;
+    const T *const x = (const T *)p.q + at * D;
+    Pack<T, 2> pairs[G][4];
+    float most = 0.0f;
+#pragma unroll
+    for (int f = 0; f < G; ++f)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int byte = WORDS * h + 4 * f + y;
+        pairs[f][y] = *(const Pack<T, 2> *)(x + 32 * (byte % G) + 2 * (byte / G));
+        most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fabsf(to_f32(pairs[f][y].v[0])),
+                                         __builtin_fabsf(to_f32(pairs[f][y].v[1]))));
+      }
+    int up = 0; // powers of two
+    if (sizeof(T) == 2 && !std::is_same<T, _Float16>::value) {
+      most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      up = 14 + 127 - (int)(__builtin_bit_cast(unsigned, most) >> 23);
+    }
+    by[r] = __builtin_ldexpf(__builtin_fabsf(scale), -up);
+#pragma unroll
+    for (int f = 0; f < G; ++f) {
+      constexpr int order[4] = {0, 2, 1, 3};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = to_f32(pairs[f][order[e % 4]].v[e / 4]);
+        q[r][f][e] = (_Float16)__builtin_ldexpf(scale < 0.0f ? -v : v, up);
+      }
+    }
+  }
+
+  v4f o[2][2 * G];
+  float top[2], sum[2];
+  unsigned nan[2] = {0, 0}; // groups of the result that are NaN
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    top[r] = -inf;
+    sum[r] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2 * G; ++t)
+      o[r][t] = v4f{0, 0, 0, 0};
+  }
+
+  // The wave makes 16 of a tile's keys, those from 16 wave on; lane l knows where
+  // those of the tile `known_from` + l lie, as the cache's row of the first.
+  constexpr unsigned kNowhere = ~0u;
+  unsigned place = kNowhere;
+  int known_from = 0;
+  auto find_places = [&](int from) {
+    known_from = from;
+    const unsigned key = (unsigned)(tile + from + lane) * 64 + 16 * wave;
+    place = kNowhere;
+    if (key < (unsigned)capacity) {
+      unsigned page = (unsigned)b, slot = key;
+      if (p.c.table) {
+        const unsigned at = key / page_size;
+        page = (unsigned)p.c.table[b * p.c.table_pages + at];
+        slot = key - at * page_size;
+      }
+      if (page < (uint64_t)p.c.pages)
+        place = (page * (unsigned)p.c.H + (unsigned)head) * page_size + slot;
+    }
+  };
+  // What a lane makes: the quarter h of key c, and of the keys 4 h + i the words
+  // c + 16 e.
+  struct Raw {
+    unsigned k[G], kp[G], v[4][ITEMS], vp[4][SG];
+    bool known;
+  } raw;
+  auto load = [&](int j) {
+    if (j - known_from >= 64)
+      find_places(j);
+    const unsigned found = __builtin_amdgcn_readlane(place, j - known_from);
+    raw.known = found != kNowhere;
+    const int64_t row = raw.known ? found : 0;
+    int room = capacity - ((tile + j) * 64 + 16 * wave);
+    room = !raw.known ? 0 : room < 16 ? room : 16; // (whole pages hold all 16)
+    auto part = [&](const void *base, int row_bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(
+          (void *)((const char *)base + row * row_bytes), 0, room * row_bytes, 0x00020000);
+    };
+    const auto kc = part(p.c.k_codes, 16 * G), vc = part(p.c.v_codes, 16 * G);
+    const auto kp = part(p.c.k_scales, 4 * G), vp = part(p.c.v_scales, 4 * G);
+    load_words<G>(kc, c * (16 * G) + h * (4 * G), raw.k);
+    load_words<G>(kp, c * (4 * G), raw.kp);
+    const int word = WORDS < 16 ? c % WORDS : c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int e = 0; e < ITEMS; ++e)
+        load_words<1>(vc, (4 * h + i) * (16 * G) + 4 * (word + 16 * e), *(unsigned(*)[1])&raw.v[i][e]);
+      load_words<SG>(vp, (4 * h + i) * (4 * G) + (4 * word) % G * 4, raw.vp[i]);
+    }
+  };
+
+  // careful: some scale or lowest value is not finite, or what they give too large.
+  auto make_keys = [&](auto careful) {
+    v2h s[G], m[G]; // of the groups of bytes x, x + 2
+#pragma unroll
+    for (int x = 0; x < G; ++x) {
+      const unsigned one = raw.kp[x], other = raw.kp[(x + 2) % G];
+      s[x] = halves_of(low_halves(one, other)), m[x] = halves_of(high_halves(one, other));
+    }
+#pragma unroll
+    for (int f = 0; f < G; ++f) {
+      const unsigned w = raw.k[f];
+      const int x = 4 * f % G, x1 = (4 * f + 1) % G;
+      v2h v[4] = {__builtin_elementwise_fma(codes_of<true>(w), s[x], m[x]),
+          __builtin_elementwise_fma(codes_of<true>(w >> 8), s[x1], m[x1]),
+          __builtin_elementwise_fma(codes_of<false>(w), s[x], m[x]),
+          __builtin_elementwise_fma(codes_of<false>(w >> 8), s[x1], m[x1])};
+      if (careful.value) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = within(v[i]);
+          const int g = i % 2 ? x1 : x;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!is_finite(s[g][e]) || !is_finite(m[g][e]))
+              v[i][e] = (_Float16)__builtin_nanf("");
+        }
+      }
+      *(v8h *)(keys + ((wave * G + f) * 64 + lane) * 16) =
+          v8h{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+    }
+  };
+  auto make_values = [&](auto careful, unsigned *marked) {
+    v2h s[2][SG], m[2][SG]; // of keys 4 h + 2 i and the next
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int g = 0; g < SG; ++g) {
+        const unsigned one = raw.vp[2 * i][g], other = raw.vp[2 * i + 1][g];
+        s[i][g] = halves_of(low_halves(one, other)), m[i][g] = halves_of(high_halves(one, other));
+        if (careful.value) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!is_finite(s[i][g][e]) || !is_finite(m[i][g][e])) {
+              s[i][g][e] = m[i][g][e] = 0;
+              const int all = G > 4 ? 4 * c % G + g : g;
+              atomicOr(marked + 16 * wave + 4 * h + 2 * i + e, 1u << all);
+            }
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < ITEMS; ++e) {
+      v2h v[8][2]; // [z][keys]
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const unsigned one = raw.v[2 * i][e], other = raw.v[2 * i + 1][e];
+        const unsigned w[2] = {low_halves(one, other), high_halves(one, other)};
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const unsigned at = w[y / 2] >> (8 * (y % 2));
+          v[2 * y][i] = __builtin_elementwise_fma(codes_of<true>(at), s[i][y % SG], m[i][y % SG]);
+          v[2 * y + 1][i] = __builtin_elementwise_fma(codes_of<false>(at), s[i][y % SG], m[i][y % SG]);
+          if (careful.value)
+            v[2 * y][i] = within(v[2 * y][i]), v[2 * y + 1][i] = within(v[2 * y + 1][i]);
+        }
+      }
+      if (WORDS < 16 && c >= WORDS)
+        continue;
+#pragma unroll
+      for (int z = 0; z < 8; ++z) {
+        const int element = z * WORDS + c + 16 * e;
+        uint8_t *const to = values +
+            (((wave / 2) * (2 * G) + element / 16) * 64 + h * 16 + element % 16) * 16 + wave % 2 * 8;
+        typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+        *(v4h *)to = v4h{v[z][0][0], v[z][0][1], v[z][1][0], v[z][1][1]};
+      }
+    }
+  };
+  auto make = [&](int parity) {
+    // (a code is at most 15: if 15 s + m is finite, so is what lies between)
+    v2h worst = {0, 0};
+    auto look = [&](unsigned one, unsigned other) {
+      const v2h s = halves_of(low_halves(one, other)), m = halves_of(high_halves(one, other));
+      worst = __builtin_elementwise_fma(
+          __builtin_elementwise_fma(s, v2h{15, 15}, m), v2h{0, 0}, worst);
+    };
+#pragma unroll
+    for (int g = 0; g < G; g += 2)
+      look(raw.kp[g], raw.kp[g + 1]);
+    const bool k_careful = !(worst[0] == 0) || !(worst[1] == 0);
+    worst = v2h{0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int g = 0; g < SG; ++g)
+        look(raw.vp[2 * i][g], raw.vp[2 * i + 1][g]);
+    const bool v_careful = !(worst[0] == 0) || !(worst[1] == 0);
+    unsigned *const marked = marks + 64 * parity;
+    if (!raw.known && lane < 16)
+      atomicOr(marked + 16 * wave + lane, kUnknown);
+    if (__any(k_careful))
+      make_keys(std::true_type{});
+    else
+      make_keys(std::false_type{});
+    if (__any(v_careful))
+      make_values(std::true_type{}, marked);
+    else
+      make_values(std::false_type{}, marked);
+  };
+
+  // masked: some rows do not see some of the keys, or some are marked.
+  auto work = [&](int key0, int parity, auto masked) {
+    v4f s[2][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        s[r][u] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int f = 0; f < G; ++f) {
+        const v8h k = *(const v8h *)(keys + ((u * G + f) * 64 + lane) * 16);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[r][f], s[r][u], 0, 0, 0);
+      }
+    }
+    unsigned seen[2] = {0, 0}; // bit 4 u + i
+    if (masked.value) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const v4u mark = *(const v4u *)(marks + 64 * parity + 16 * u + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 16 * u + 4 * h + i;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool sees = !(mark[i] & kUnknown) && key >= row_lo[r] && key < row_hi[r];
+            seen[r] |= sees ? 1u << (4 * u + i) : 0u;
+            nan[r] |= sees ? mark[i] : 0u;
+            s[r][u][i] = sees ? s[r][u][i] : -inf;
+          }
+        }
+      }
+    }
+    // maxima, as above
+    float most[2];
+    bool grown = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float m = s[r][0][0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j)
+        m = __builtin_fmaxf(m, s[r][j / 4][j % 4]);
+      most[r] = m == -inf ? m : m * by[r];
+      grown = grown || most[r] > top[r] + 8.0f;
+    }
+    if (__any(grown)) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float m = __builtin_fmaxf(most[r], __shfl_xor(most[r], 16));
+        m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+        m = __builtin_fmaxf(m, top[r]);
+        const float less = m == top[r] ? 1.0f : __builtin_amdgcn_exp2f(top[r] - m);
+        top[r] = m;
+        sum[r] *= less;
+#pragma unroll
+        for (int t = 0; t < 2 * G; ++t)
+          o[r][t] *= less;
+      }
+    }
+    v8h weights[2][2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float base = top[r] == -inf ? 0.0f : 7.0f - top[r]; // -inf: no key seen so far
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) {
+        float e[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = j + k;
+          e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][at / 4][at % 4], by[r], base));
+          if (masked.value)
+            e[k] = seen[r] >> at & 1 ? e[k] : 0.0f;
+          sum[r] += e[k];
+        }
+        typedef float v2f __attribute__((ext_vector_type(2)));
+        const v2h w = __builtin_convertvector(v2f{e[0], e[1]}, v2h);
+        weights[r][j / 8][j % 8] = w[0], weights[r][j / 8][j % 8 + 1] = w[1];
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int t = 0; t < 2 * G; ++t) {
+        const v8h v = *(const v8h *)(values + ((half * (2 * G) + t) * 64 + lane) * 16);
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, weights[r][half], o[r][t], 0, 0, 0);
+      }
+  };
+
+  if (threadIdx.x < 128)
+    marks[threadIdx.x] = 0;
+  if (tiles > 0) {
+    find_places(0);
+    load(0);
+  }
+  for (int j = 0; j < tiles; ++j) {
+    const int parity = j & 1, key0 = (tile + j) * 64;
+    gemm::lds_barrier(); // the last tile has been read
+    make(parity);
+    if (j + 1 < tiles)
+      load(j + 1);
+    gemm::lds_barrier();
+    // (the other marks were read before the last barrier but one)
+    if (threadIdx.x < 64)
+      marks[64 * (1 - parity) + threadIdx.x] = 0;
+    if (key0 >= hi || key0 + 64 <= lo)
+      continue;
+    if (key0 >= all_lo && key0 + 64 <= all_hi && !__any(marks[64 * parity + lane] != 0))
+      work(key0, parity, std::false_type{});
+    else
+      work(key0, parity, std::true_type{});
+  }
+
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    sum[r] += __shfl_xor(sum[r], 16);
+    sum[r] += __shfl_xor(sum[r], 32);
+    nan[r] |= __shfl_xor(nan[r], 16);
+    nan[r] |= __shfl_xor(nan[r], 32);
+  }
+  // Element 4 h + i of tile t is z (4 G) + j.
+  auto element_of = [&](int t, int i, int &g) {
+    const int element = 16 * t + 4 * h + i, z = element / WORDS, j = element % WORDS;
+    const int byte = 4 * j + z / 2;
+    g = byte % G;
+    return 32 * g + 2 * (byte / G) + z % 2;
+  };
+  if (p.splits > 1) {
+    const int64_t part0 = ((int64_t)bh * p.groups + group) * p.splits + split;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int mr = 32 * wave + 16 * r + c;
+      if (row0 + mr >= rows)
+        continue;
+      const int64_t part = part0 * kPromptRows + mr;
+#pragma unroll
+      for (int t = 0; t < 2 * G; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          int g;
+          const int d = element_of(t, i, g);
+          p.parts[part * D + d] = nan[r] >> g & 1 ? __builtin_nanf("") : o[r][t][i];
+        }
+      if (h == 0) {
+        float *const st = p.parts +
+            (int64_t)p.B * p.c.H * p.groups * p.splits * kPromptRows * D + part * 2;
+        st[0] = top[r];
+        st[1] = sum[r];
+      }
+    }
+    return;
+  }
+  // Results leave by way of LDS, so that a store takes whole pieces of rows.
+  __syncthreads();
+  uint8_t *const mine = (uint8_t *)shared + wave * (32 * PITCH);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const float over = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+#pragma unroll
+    for (int t = 0; t < 2 * G; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        int g;
+        const int d = element_of(t, i, g);
+        *(T *)(mine + (16 * r + c) * PITCH + 2 * d) =
+            from_f32<T>(nan[r] >> g & 1 ? __builtin_nanf("") : o[r][t][i] * over);
+      }
+  }
+  __syncthreads();
+  for (int at = lane; at < 32 * (D / 8); at += 64) {
+    const int mr = at / (D / 8), d = at % (D / 8) * 8, row = row0 + 32 * wave + mr;
+    if (row >= rows)
+      break;
+    const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
+    const int64_t to = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
+                                     : ((int64_t)b * p.S + i) * p.heads + qh;
+    *(Pack<T, 8> *)((T *)p.y + to * D + d) = *(const Pack<T, 8> *)(mine + mr * PITCH + 2 * d);
+  }
+}
+
 // The parts of a row's keys joined, a block a row: thread t weighs part t (there
 // are at most 256), then thread (s, d) sums elements 4 d .. of every part s, s +
 // across, .., and those sums meet in LDS.
@@ -759,18 +1278,22 @@ __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, in
   *(Pack<T, 4> *)((T *)p.y + at * D + 4 * d) = out;
 }
 
-// How rows are dealt to waves: tiles of 16, or of 16 / G where that takes one
-// tile (D = 64, 128, 256) or two (64, 128).
+// How rows are dealt: tiles of 16 a wave, or of 16 / G where that takes one tile
+// (D = 64, 128, 256) or two (64, 128); or 128 rows a block, once there are as many
+// (128 rows a head, tiles / blocks: 4096 keys 31 / 27 us, 1100 keys 39 / 33;
+// 2048 rows a head and 2500 keys 104 / 74).
 struct Shape {
-  bool packed;
-  int tiles, rows; // tiles of a wave; rows of a tile
+  enum { kTiles, kPacked, kPrompt } form;
+  int tiles, rows; // tiles of a unit of blocks; rows of a tile
 };
 Shape shape_of(const Attention4 &a) {
   const int64_t n = a.S * (a.heads / a.c.H);
   const int G = a.c.D / kCacheGroup;
   if (16 % G == 0 && n <= (G <= 4 ? 2 : 1) * (16 / G))
-    return {true, n > 16 / G ? 2 : 1, 16 / G};
-  return {false, n > 16 && G <= 4 ? 2 : 1, 16};
+    return {Shape::kPacked, n > 16 / G ? 2 : 1, 16 / G};
+  if (a.kind != kF32 && 16 % G == 0 && n >= kPromptRows)
+    return {Shape::kPrompt, kPromptRows / 16, 16};
+  return {Shape::kTiles, n > 16 && G <= 4 ? 2 : 1, 16};
 }
 int64_t row_groups(const Attention4 &a) {
   const Shape s = shape_of(a);
@@ -800,15 +1323,40 @@ hipError_t attend(hipStream_t st, const Arguments &p) {
   return e;
 }
 
+template <typename T, int G> hipError_t attend_prompt(hipStream_t st, const Arguments &p) {
+  // (keys, values and marks; then 128 rows of 64 G + 16 bytes)
+  constexpr int kLds = 8192 * G + 2048;
+  auto *const kernel = k_cache_prompt<T, G>;
+  if (kLds > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void *)kernel,
+        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (e != hipSuccess)
+      return e;
+  }
+  const int64_t units = (int64_t)p.B * p.c.H * p.groups;
+  kernel<<<dim3((unsigned)(units * p.splits)), 256, kLds, st>>>(p);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.splits > 1) {
+    k_cache_join<T><<<dim3((unsigned)(units * kPromptRows)), 256, 0, st>>>(
+        p, 32 * G, kPromptRows);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
 template <typename T, int G>
 hipError_t attend_group(hipStream_t st, const Arguments &p, const Shape &s) {
+  if constexpr (16 % G == 0 && sizeof(T) == 2) {
+    if (s.form == Shape::kPrompt)
+      return attend_prompt<T, G>(st, p);
+  }
   if constexpr (16 % G == 0) {
-    if (s.packed && s.tiles == 1)
+    if (s.form == Shape::kPacked && s.tiles == 1)
       return attend<T, G, 1, true>(st, p);
   }
   if constexpr (G <= 4) {
     if constexpr (16 % G == 0) {
-      if (s.packed)
+      if (s.form == Shape::kPacked)
         return attend<T, G, 2, true>(st, p);
     }
     if (s.tiles > 1)

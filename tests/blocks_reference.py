@@ -93,10 +93,11 @@ def rows_of(pages, table, b):
     return np.concatenate(list(one), axis=1)
 
 
-def attention(q, cache, past, table=None, counts=None, starts=None, scale=None, causal=True, window=0):
+def attention(q, cache, past, table=None, counts=None, starts=None, scale=None, causal=True, window=0, half=False):
     """(y, sure): q [B, Hq, S, D]; rows behind a sequence's tokens are NaN.  sure:
     for each result the magnitudes its rounding errors are measured by, (largest
-    sum |q khat| scale, largest |vhat|, largest code * scale of v, keys seen)."""
+    sum |q khat| scale, largest |vhat|, largest code * scale of v, keys seen).
+    half: khat and vhat are the nearest f16, +-65504 at most."""
     kc, ks, vc, vs = cache
     B, Hq, S, D = q.shape
     H = kc.shape[1]
@@ -106,6 +107,8 @@ def attention(q, cache, past, table=None, counts=None, starts=None, scale=None, 
     for b in range(B):
         n = S if counts is None else int(counts[b])
         K, V = values4(rows_of(kc, table, b), rows_of(ks, table, b)), values4(rows_of(vc, table, b), rows_of(vs, table, b))
+        if half:
+            K, V = (np.clip(x, -65504, 65504).astype(np.float16).astype(np.float64) for x in (K, V))
         vsc = np.abs(rows_of(vs, table, b).astype(np.float64))
         for i in range(n):
             t = int(past[b]) + i

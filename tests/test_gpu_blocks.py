@@ -531,6 +531,131 @@ def test_attention_of_sharp_and_flat_scores(om):
         check_attention(om, got, want, sure, "f32")
 
 
+def check_prompt(got, want, sure, dtype):
+    """Against f16(khat) and f16(vhat): scores, weights and sums as in check_attention,
+    weights rounded to f16 (2^-11) in place of split ones; what f16 drops of a bf16
+    query is 2^-39 of its largest element."""
+    score = 300 * 2.0 ** -24 * (1 + sure[..., 0]) + 2.0 ** -22
+    off = (2 * score + 2.0 ** -11) * sure[..., 1] + (sure[..., 3] + 64) * 2.0 ** -24 * sure[..., 2]
+    seen = ~np.isnan(want)
+    limit = off[..., None] + ref.half_step(dtype) * np.abs(want) * (1 + 2.0 ** -7) + ref.smallest_step(dtype)
+    assert np.all(np.abs(got - want)[seen] <= limit[seen]), (np.abs(got - want) / limit)[seen].max()
+
+
+PROMPTS = [
+    # B, Hq, H, S, D, page size, paged, past, options: 128 rows of a head and more
+    (1, 4, 1, 40, 128, 16, True, [0], {}),
+    (2, 8, 2, 33, 64, 48, True, [100, 3], {}),
+    (1, 8, 1, 17, 256, 64, True, [50], {}),
+    (2, 2, 2, 150, 128, 301, False, [77, 0], {}),
+    (2, 4, 2, 150, 64, 301, False, [151, 0], {"counts": [150, 0]}),
+    (2, 2, 2, 130, 128, 64, True, [5, 400], {"counts": [3, 129]}),
+    (1, 2, 1, 70, 128, 16, True, [65], {"window": 20}),
+    (1, 2, 1, 70, 256, 16, True, [30], {"causal": 0}),
+    (2, 2, 1, 64, 64, 32, True, [10, 20], {"starts": [60, 5]}),
+    (2, 2, 1, 64, 128, 32, True, [10, 10], {"starts": [90, 3], "causal": 0}),
+    (1, 7, 1, 30, 128, 16, True, [300], {"scale": -1.5}),
+    (1, 7, 1, 30, 64, 16, True, [70], {"scale": 0.0}),
+    (1, 64, 1, 2, 128, 16, True, [3000], {}),
+    (5, 26, 13, 64, 64, 16, True, [0, 1, 17, 64, 128], {}),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads_first", [True, False])
+@pytest.mark.parametrize("case", range(len(PROMPTS)))
+def test_attention_of_prompts(om, case, heads_first, dtype):
+    B, Hq, H, S, D, size, paged, past, options = PROMPTS[case]
+    rng = np.random.default_rng(100 + case)
+    each = max(p + S - 1 for p in past) // size + 2 if paged else 1
+    table = tables_of(rng, B, each) if paged else None
+    c = random_cache(om, rng, B * each + 1, H, size, D)
+    counts = options.get("counts")
+    for b in range(B):  # as in test_attention
+        n = past[b] + (S if counts is None else counts[b])
+        for t in range(n, each * size):
+            page = table[b, t // size] if paged else b
+            c.k_scales[page, :, t % size] = np.nan
+            c.v_scales[page, :, t % size] = np.inf
+        if paged:
+            table[b, -(-n // size):] = [-1, 10 ** 6][b % 2]
+    q = om.from_float32(rng.standard_normal((B, Hq, S, D)), dt(om, dtype))
+    arrays = {k: np.array(v, np.int32) for k, v in options.items() if k in ("counts", "starts")}
+    scale = np.float32(options["scale"]) if "scale" in options else None
+    kinds = dict(causal=options.get("causal", 1), window=options.get("window", 0))
+    want, sure = ref.attention(om.to_float32(q), c.tensors, past, None if table is None else np.clip(table, 0, B * each),
+                               arrays.get("counts"), arrays.get("starts"), scale, half=True, **kinds)
+    out = on(om, pack_heads(om.from_float32(np.full(q.shape, 77.0), dt(om, dtype)), heads_first))
+    om.CacheAttention4(on(om, pack_heads(q, heads_first)), to_gpu(om, c), on(om, np.array(past, np.int32)),
+                       None if table is None else on(om, table), scale=None if scale is None else on(om, scale), out=out,
+                       **{k: on(om, v) for k, v in arrays.items()}, **kinds)
+    got = unpack_heads(back(om, out), Hq, heads_first)
+    assert np.array_equal(got[np.isnan(want)], np.full(np.isnan(want).sum(), 77.0, np.float32))  # rows behind the last token
+    assert np.isfinite(got).all()
+    check_prompt(got, want, sure, dtype)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_of_prompts_nan_where_it_is_seen(om, D):
+    """A key's NaN reaches the rows that see it; a value's, of them, the elements of
+    its group; neither any row before."""
+    rng = np.random.default_rng(3)
+    c = random_cache(om, rng, 2, 1, 200, D)
+    c.v_scales[0, 0, 100, 1, 0] = np.inf
+    c.v_scales[0, 0, 131, 0, 1] = np.nan
+    c.k_scales[0, 0, 150, 1, 1] = np.nan
+    q = om.from_float32(rng.standard_normal((2, 1, 200, D)), om.bfloat16)
+    got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.zeros(2, np.int32))))
+    nan = np.zeros(got.shape, bool)
+    nan[0, 0, 100:, 32:64] = True
+    nan[0, 0, 131:, :32] = True
+    nan[0, 0, 150:] = True
+    assert np.array_equal(np.isnan(got), nan)
+    want, sure = ref.attention(om.to_float32(q)[:, :, :100], c.tensors, [0, 0], half=True)
+    check_prompt(got[:, :, :100], want, sure, "bf16")
+
+
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -20, 2.0 ** 60])
+def test_attention_of_prompts_of_any_magnitude(om, size):
+    """bf16 queries beyond f16's range, their elements 2^8 apart, with the scale that
+    takes them back; caches whose values are the largest that it holds, and small ones."""
+    rng = np.random.default_rng(4)
+    S, D = 140, 128
+    q = rng.standard_normal((1, 1, S, D)) * np.exp2(rng.integers(-8, 1, D)) * size
+    q = om.from_float32(q.astype(np.float32), om.bfloat16)
+    c = om.Cache4(1, 1, S, D)
+    k = rng.standard_normal((1, 1, S, D)).astype(np.float32)
+    v = rng.standard_normal((1, 1, S, D)).astype(np.float32)
+    v[:, :, :, :32] = np.where(rng.random((1, 1, S, 32)) < 0.5, 65504, -65504)
+    v[:, :, :, 32:64] *= 1e-6
+    c.k_codes, c.k_scales = ref.quantize4(k)
+    c.v_codes, c.v_scales = ref.quantize4(v)
+    scale = np.float32(0.3 / size)
+    got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.zeros(1, np.int32)), scale=on(om, scale)))
+    want, sure = ref.attention(om.to_float32(q), c.tensors, [0], scale=scale, half=True)
+    for d in range(0, D, 32):  # by groups: of their own magnitudes
+        sure[..., 1:3] = [[65504, 131008], [4e-6, 1e-5], [5, 10], [5, 10]][d // 32]
+        check_prompt(got[..., d:d + 32], want[..., d:d + 32], sure, "bf16")
+
+
+def test_attention_of_prompts_of_sharp_and_flat_scores(om):
+    """As test_attention_of_sharp_and_flat_scores."""
+    rng = np.random.default_rng(2)
+    D, n = 128, 300
+    k = rng.standard_normal((1, 1, n, D)).astype(np.float32)
+    k *= np.linspace(0.01, 20, n, dtype=np.float32)[None, None, :, None]
+    v = rng.standard_normal((1, 1, n, D)).astype(np.float32)
+    q = np.concatenate([k[:, :, -1:] * 0.3, k[:, :, :1] * 100, -k[:, :, -1:]], 1)
+    q = om.from_float32(np.repeat(q, 60, 2).astype(np.float32), np.dtype(np.float16))
+    for order in (1, -1):
+        c = om.Cache4(1, 1, n, D)
+        c.k_codes, c.k_scales = ref.quantize4(k[:, :, ::order])
+        c.v_codes, c.v_scales = ref.quantize4(v)
+        got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.array([n - 60], np.int32)), causal=0))
+        want, sure = ref.attention(om.to_float32(q), c.tensors, [n - 60], causal=False, half=True)
+        check_prompt(got, want, sure, "f16")
+
+
 def test_a_decoder_layers_attention_block(om):
     """The ops as a decoder uses them, two prompts of different lengths and then two
     more tokens of each: every step against what its own inputs say."""
