@@ -311,9 +311,9 @@ void om_mi355x_CacheAppend4(OMTensor *k_codes, OMTensor *k_scales,
  * see, NaN or infinite, does not reach its result.  Rows i >= counts[b] of y
  * stay as they were.
  * Sums, scores and statistics are f32, weights are held to 2^-16 for y of 16 bits
- * and 2^-23 for f32; but where y has 16 bits, D is 64, 128 or 256 and a head of
- * the cache has 128 rows or more (S * Hq / H), khat, vhat and the weights are
- * rounded to f16 (khat and vhat limited to +-65504). */
+ * and 2^-23 for f32; but where y is bf16, D is 64, 128 or 256 and a head of the
+ * cache has 128 rows or more (S * Hq / H), khat, vhat and the weights are rounded
+ * to f16 (khat and vhat limited to +-65504). */
 void om_mi355x_CacheAttention4(OMTensor *y, const OMTensor *q,
     const OMTensor *k_codes, const OMTensor *k_scales,
     const OMTensor *v_codes, const OMTensor *v_scales,

@@ -698,15 +698,17 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
 // ---------------------------------------------------------------------------
 // attention of many rows
 // ---------------------------------------------------------------------------
-// Where a head of keys has many rows, and their type 16 bits, what bounds the
-// kernel above is scaling and splitting weights anew in every wave.  Here a block
-// of 128 rows makes 64 keys and values at a time into f16 in LDS, s c + m with one
-// rounding (2^-11; what lies beyond 65504, up to which rows are stored, becomes
-// that), and its waves multiply those by q, which f16 holds (bf16 ones with each
-// row's largest at 2^14, so that what f16 drops of others is 2^-38 of it), and by p
-// in f16 (2^-11 again), 2^7 times what it is relative to a maximum that is at most 8
-// powers of two behind: what f16 loses of p is below 2^-32 of the largest.  Sums,
-// scores and statistics are f32.
+// Where a head of keys has many rows, what bounds the kernel above is scaling and
+// splitting weights anew in every wave.  Here a block of 128 rows makes 64 keys and
+// values at a time into f16 in LDS, s c + m with one rounding (2^-11; what lies
+// beyond 65504, up to which rows are stored, becomes that), and its waves multiply
+// those by q, which f16 holds with each row's largest at 2^14 (what it drops of
+// others is 2^-38 of it), and by p in f16 (2^-11 again), 2^7 times what it is
+// relative to a maximum that is at most 8 powers of two behind: what f16 loses of p
+// is below 2^-32 of the largest.  Sums, scores and statistics are f32.  Results in
+// bf16, whose own rounding is 2^-8, are as near to the exact ones as the tiles'
+// (0.0018 and 0.0017 of their magnitude); f16's, 2^-11, would be off by up to three
+// times as much (0.0006 and 0.0002), so those and f32's stay with the tiles.
 //
 // A wave has 32 rows in two tiles: both operands that it reads from LDS, 1 KB each,
 // feed two instructions, which is as fast as LDS can feed four waves.  Scores'
@@ -749,8 +751,9 @@ __device__ __forceinline__ bool is_finite(_Float16 x) {
   return (__builtin_bit_cast(unsigned short, x) & 0x7C00) != 0x7C00;
 }
 
-template <typename T, int G>
+template <int G>
 __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Arguments p) {
+  typedef __bf16 T;
   constexpr int D = 32 * G, WORDS = 4 * G, ITEMS = (WORDS + 15) / 16;
   constexpr int SG = G < 4 ? G : 4; // groups of a word's bytes
   constexpr int PITCH = 2 * D + 16; // of a row of results in LDS
@@ -840,13 +843,11 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
         most = __builtin_fmaxf(most, __builtin_fmaxf(__builtin_fabsf(to_f32(pairs[f][y].v[0])),
                                          __builtin_fabsf(to_f32(pairs[f][y].v[1]))));
       }
-    int up = 0; // powers of two
-    if (sizeof(T) == 2 && !std::is_same<T, _Float16>::value) {
-      most = __builtin_fmaxf(most, __shfl_xor(most, 16));
-      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
-      up = 14 + 127 - (int)(__builtin_bit_cast(unsigned, most) >> 23);
-    }
-    by[r] = __builtin_ldexpf(__builtin_fabsf(scale), -up);
+    most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+    most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+    const int up = 14 + 127 - (int)(__builtin_bit_cast(unsigned, most) >> 23);
+    // (not 0: what is not seen has the score -inf)
+    by[r] = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale), -up), 0x1p-126f);
 #pragma unroll
     for (int f = 0; f < G; ++f) {
       constexpr int order[4] = {0, 2, 1, 3};
@@ -1032,7 +1033,7 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
   };
 
   // masked: some rows do not see some of the keys, or some are marked.
-  auto work = [&](int key0, int parity, auto masked) {
+  auto work = [&](int key0, int parity, bool masked) {
     v4f s[2][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -1047,8 +1048,7 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
           s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[r][f], s[r][u], 0, 0, 0);
       }
     }
-    unsigned seen[2] = {0, 0}; // bit 4 u + i
-    if (masked.value) {
+    if (masked) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const v4u mark = *(const v4u *)(marks + 64 * parity + 16 * u + 4 * h);
@@ -1058,7 +1058,6 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const bool sees = !(mark[i] & kUnknown) && key >= row_lo[r] && key < row_hi[r];
-            seen[r] |= sees ? 1u << (4 * u + i) : 0u;
             nan[r] |= sees ? mark[i] : 0u;
             s[r][u][i] = sees ? s[r][u][i] : -inf;
           }
@@ -1074,7 +1073,7 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
 #pragma unroll
       for (int j = 1; j < 16; ++j)
         m = __builtin_fmaxf(m, s[r][j / 4][j % 4]);
-      most[r] = m == -inf ? m : m * by[r];
+      most[r] = m * by[r];
       grown = grown || most[r] > top[r] + 8.0f;
     }
     if (__any(grown)) {
@@ -1102,8 +1101,6 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
         for (int k = 0; k < 2; ++k) {
           const int at = j + k;
           e[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][at / 4][at % 4], by[r], base));
-          if (masked.value)
-            e[k] = seen[r] >> at & 1 ? e[k] : 0.0f;
           sum[r] += e[k];
         }
         typedef float v2f __attribute__((ext_vector_type(2)));
@@ -1140,10 +1137,8 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
       marks[64 * (1 - parity) + threadIdx.x] = 0;
     if (key0 >= hi || key0 + 64 <= lo)
       continue;
-    if (key0 >= all_lo && key0 + 64 <= all_hi && !__any(marks[64 * parity + lane] != 0))
-      work(key0, parity, std::false_type{});
-    else
-      work(key0, parity, std::true_type{});
+    work(key0, parity, key0 < all_lo || key0 + 64 > all_hi ||
+                           __any(marks[64 * parity + lane] != 0));
   }
 
 #pragma unroll
@@ -1279,8 +1274,8 @@ __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, in
 }
 
 // How rows are dealt: tiles of 16 a wave, or of 16 / G where that takes one tile
-// (D = 64, 128, 256) or two (64, 128); or 128 rows a block, once there are as many
-// (128 rows a head, tiles / blocks: 4096 keys 31 / 27 us, 1100 keys 39 / 33;
+// (D = 64, 128, 256) or two (64, 128); or bf16's 128 rows a block, once there are
+// as many (128 rows a head, tiles / blocks: 4096 keys 31 / 27 us, 1100 keys 39 / 33;
 // 2048 rows a head and 2500 keys 104 / 74).
 struct Shape {
   enum { kTiles, kPacked, kPrompt } form;
@@ -1291,7 +1286,7 @@ Shape shape_of(const Attention4 &a) {
   const int G = a.c.D / kCacheGroup;
   if (16 % G == 0 && n <= (G <= 4 ? 2 : 1) * (16 / G))
     return {Shape::kPacked, n > 16 / G ? 2 : 1, 16 / G};
-  if (a.kind != kF32 && 16 % G == 0 && n >= kPromptRows)
+  if (a.kind == kBF16 && 16 % G == 0 && n >= kPromptRows)
     return {Shape::kPrompt, kPromptRows / 16, 16};
   return {Shape::kTiles, n > 16 && G <= 4 ? 2 : 1, 16};
 }
@@ -1323,10 +1318,10 @@ hipError_t attend(hipStream_t st, const Arguments &p) {
   return e;
 }
 
-template <typename T, int G> hipError_t attend_prompt(hipStream_t st, const Arguments &p) {
+template <int G> hipError_t attend_prompt(hipStream_t st, const Arguments &p) {
   // (keys, values and marks; then 128 rows of 64 G + 16 bytes)
   constexpr int kLds = 8192 * G + 2048;
-  auto *const kernel = k_cache_prompt<T, G>;
+  auto *const kernel = k_cache_prompt<G>;
   if (kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void *)kernel,
         hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
@@ -1337,7 +1332,7 @@ template <typename T, int G> hipError_t attend_prompt(hipStream_t st, const Argu
   kernel<<<dim3((unsigned)(units * p.splits)), 256, kLds, st>>>(p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.splits > 1) {
-    k_cache_join<T><<<dim3((unsigned)(units * kPromptRows)), 256, 0, st>>>(
+    k_cache_join<__bf16><<<dim3((unsigned)(units * kPromptRows)), 256, 0, st>>>(
         p, 32 * G, kPromptRows);
     e = hipGetLastError();
   }
@@ -1346,9 +1341,9 @@ template <typename T, int G> hipError_t attend_prompt(hipStream_t st, const Argu
 
 template <typename T, int G>
 hipError_t attend_group(hipStream_t st, const Arguments &p, const Shape &s) {
-  if constexpr (16 % G == 0 && sizeof(T) == 2) {
+  if constexpr (16 % G == 0 && std::is_same<T, __bf16>::value) {
     if (s.form == Shape::kPrompt)
-      return attend_prompt<T, G>(st, p);
+      return attend_prompt<G>(st, p);
   }
   if constexpr (16 % G == 0) {
     if (s.form == Shape::kPacked && s.tiles == 1)

@@ -561,7 +561,7 @@ PROMPTS = [
 ]
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("heads_first", [True, False])
 @pytest.mark.parametrize("case", range(len(PROMPTS)))
 def test_attention_of_prompts(om, case, heads_first, dtype):
@@ -584,7 +584,7 @@ def test_attention_of_prompts(om, case, heads_first, dtype):
     scale = np.float32(options["scale"]) if "scale" in options else None
     kinds = dict(causal=options.get("causal", 1), window=options.get("window", 0))
     want, sure = ref.attention(om.to_float32(q), c.tensors, past, None if table is None else np.clip(table, 0, B * each),
-                               arrays.get("counts"), arrays.get("starts"), scale, half=True, **kinds)
+                               arrays.get("counts"), arrays.get("starts"), scale, half=dtype == "bf16", **kinds)
     out = on(om, pack_heads(om.from_float32(np.full(q.shape, 77.0), dt(om, dtype)), heads_first))
     om.CacheAttention4(on(om, pack_heads(q, heads_first)), to_gpu(om, c), on(om, np.array(past, np.int32)),
                        None if table is None else on(om, table), scale=None if scale is None else on(om, scale), out=out,
@@ -592,7 +592,10 @@ def test_attention_of_prompts(om, case, heads_first, dtype):
     got = unpack_heads(back(om, out), Hq, heads_first)
     assert np.array_equal(got[np.isnan(want)], np.full(np.isnan(want).sum(), 77.0, np.float32))  # rows behind the last token
     assert np.isfinite(got).all()
-    check_prompt(got, want, sure, dtype)
+    if dtype == "bf16":
+        check_prompt(got, want, sure, dtype)
+    else:
+        check_attention(om, got, want, sure, dtype)
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
@@ -646,14 +649,14 @@ def test_attention_of_prompts_of_sharp_and_flat_scores(om):
     k *= np.linspace(0.01, 20, n, dtype=np.float32)[None, None, :, None]
     v = rng.standard_normal((1, 1, n, D)).astype(np.float32)
     q = np.concatenate([k[:, :, -1:] * 0.3, k[:, :, :1] * 100, -k[:, :, -1:]], 1)
-    q = om.from_float32(np.repeat(q, 60, 2).astype(np.float32), np.dtype(np.float16))
+    q = om.from_float32(np.repeat(q, 60, 2).astype(np.float32), om.bfloat16)
     for order in (1, -1):
         c = om.Cache4(1, 1, n, D)
         c.k_codes, c.k_scales = ref.quantize4(k[:, :, ::order])
         c.v_codes, c.v_scales = ref.quantize4(v)
         got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, np.array([n - 60], np.int32)), causal=0))
         want, sure = ref.attention(om.to_float32(q), c.tensors, [n - 60], causal=False, half=True)
-        check_prompt(got, want, sure, "f16")
+        check_prompt(got, want, sure, "bf16")
 
 
 def test_a_decoder_layers_attention_block(om):
