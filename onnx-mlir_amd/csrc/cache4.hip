@@ -756,7 +756,7 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
   typedef __bf16 T;
   constexpr int D = 32 * G, WORDS = 4 * G, ITEMS = (WORDS + 15) / 16;
   constexpr int SG = G < 4 ? G : 4; // groups of a word's bytes
-  constexpr int PITCH = 2 * D + 16; // of a row of results in LDS
+  constexpr int PITCH = D + 4; // of a row of results in LDS
   extern __shared__ __attribute__((aligned(16))) float shared[];
   uint8_t *const keys = (uint8_t *)shared, *const values = keys + G * 4096;
   // [parity][key]: groups of its value that are not finite, and whether it is known
@@ -771,7 +771,9 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
   const int bh = (unsigned)unit / (unsigned)p.groups;
   int group = unit - bh * p.groups;
   const int b = (unsigned)bh / (unsigned)p.c.H, head = (unsigned)bh % (unsigned)p.c.H;
-  if (p.causal) // those with the most keys first
+  // Those with the most keys first (2048 / 4096 / 4 x 2048 rows: 156 / 196 / 510 us, in
+  // order of the keys 175 / 236 / 579).
+  if (p.causal)
     group = p.groups - 1 - group;
 
   const int past = p.c.past[b];
@@ -1155,56 +1157,52 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
     g = byte % G;
     return 32 * g + 2 * (byte / G) + z % 2;
   };
-  if (p.splits > 1) {
-    const int64_t part0 = ((int64_t)bh * p.groups + group) * p.splits + split;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int mr = 32 * wave + 16 * r + c;
-      if (row0 + mr >= rows)
-        continue;
-      const int64_t part = part0 * kPromptRows + mr;
-#pragma unroll
-      for (int t = 0; t < 2 * G; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          int g;
-          const int d = element_of(t, i, g);
-          p.parts[part * D + d] = nan[r] >> g & 1 ? __builtin_nanf("") : o[r][t][i];
-        }
-      if (h == 0) {
-        float *const st = p.parts +
-            (int64_t)p.B * p.c.H * p.groups * p.splits * kPromptRows * D + part * 2;
-        st[0] = top[r];
-        st[1] = sum[r];
-      }
-    }
-    return;
-  }
   // Results leave by way of LDS, so that a store takes whole pieces of rows.
-  __syncthreads();
-  uint8_t *const mine = (uint8_t *)shared + wave * (32 * PITCH);
+  float *const mine = shared + wave * (16 * PITCH);
+  const int64_t part0 = (((int64_t)bh * p.groups + group) * p.splits + split) * kPromptRows;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    const float over = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+    const float over = p.splits > 1 ? 1.0f : sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+    gemm::lds_barrier();
 #pragma unroll
     for (int t = 0; t < 2 * G; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         int g;
         const int d = element_of(t, i, g);
-        *(T *)(mine + (16 * r + c) * PITCH + 2 * d) =
-            from_f32<T>(nan[r] >> g & 1 ? __builtin_nanf("") : o[r][t][i] * over);
+        mine[c * PITCH + d] = nan[r] >> g & 1 ? __builtin_nanf("") : o[r][t][i] * over;
       }
-  }
-  __syncthreads();
-  for (int at = lane; at < 32 * (D / 8); at += 64) {
-    const int mr = at / (D / 8), d = at % (D / 8) * 8, row = row0 + 32 * wave + mr;
-    if (row >= rows)
-      break;
-    const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
-    const int64_t to = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
-                                     : ((int64_t)b * p.S + i) * p.heads + qh;
-    *(Pack<T, 8> *)((T *)p.y + to * D + d) = *(const Pack<T, 8> *)(mine + mr * PITCH + 2 * d);
+    gemm::lds_barrier();
+    const int first = 32 * wave + 16 * r;
+#pragma unroll 2
+    for (int at = lane; at < 16 * (D / 8); at += 64) {
+      const int mr = at / (D / 8), d = at % (D / 8) * 8, row = row0 + first + mr;
+      if (row >= rows)
+        break;
+      const v4f x = *(const v4f *)(mine + mr * PITCH + d),
+                y = *(const v4f *)(mine + mr * PITCH + d + 4);
+      if (p.splits > 1) {
+        float *const to = p.parts + (part0 + first + mr) * D + d;
+        *(v4f *)to = x;
+        *(v4f *)(to + 4) = y;
+        continue;
+      }
+      const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
+      const int64_t to = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
+                                       : ((int64_t)b * p.S + i) * p.heads + qh;
+      Pack<T, 8> out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out.v[j] = from_f32<T>(x[j]), out.v[4 + j] = from_f32<T>(y[j]);
+      *(Pack<T, 8> *)((T *)p.y + to * D + d) = out;
+    }
+    if (p.splits > 1 && h == 0 && row0 + first + c < rows) {
+      float *const st = p.parts +
+          (int64_t)p.B * p.c.H * p.groups * p.splits * kPromptRows * D +
+          (part0 + first + c) * 2;
+      st[0] = top[r];
+      st[1] = sum[r];
+    }
   }
 }
 
@@ -1273,6 +1271,68 @@ __global__ __launch_bounds__(256) void k_cache_join(const Arguments p, int D, in
   *(Pack<T, 4> *)((T *)p.y + at * D + 4 * d) = out;
 }
 
+// The same where parts are few and rows many: 256 / (D / 4) rows a block, a thread
+// weighs all parts of its row and sums four elements of them.
+template <typename T>
+__global__ __launch_bounds__(256) void k_cache_join_rows(const Arguments p, int D, int tile_rows) {
+  const int lanes = D / 4;
+  const int64_t units = (int64_t)p.B * p.c.H * p.groups;
+  const int64_t id = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+  const int unit = (int)(id / tile_rows), r = (int)(id % tile_rows), d = threadIdx.x % lanes;
+  if ((int)threadIdx.x >= 256 / lanes * lanes || unit >= units)
+    return;
+  const int group = unit % p.groups, bh = unit / p.groups;
+  const int b = bh / p.c.H, head = bh % p.c.H;
+  int count = p.S;
+  if (p.c.counts) {
+    const int n = p.c.counts[b];
+    count = n < 0 ? 0 : n < p.S ? n : p.S;
+  }
+  const int row = group * tile_rows + r;
+  if (row >= count * p.per_head)
+    return;
+  const float *const stats = p.parts + units * p.splits * tile_rows * D;
+  const int64_t part0 = (int64_t)unit * p.splits * tile_rows + r;
+  const float inf = __builtin_inff();
+  float top = -inf, total = 0.0f;
+  v4f v = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s)
+    top = __builtin_fmaxf(top, stats[(part0 + (int64_t)s * tile_rows) * 2]);
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const int64_t part = part0 + (int64_t)s * tile_rows;
+    const float m = stats[part * 2];
+    const float f = m == -inf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    total += stats[part * 2 + 1] * f;
+    v += *(const v4f *)(p.parts + part * D + 4 * d) * f;
+  }
+  const float over = total == 0.0f ? 0.0f : 1.0f / total;
+  const int i = row / p.per_head, qh = head * p.per_head + row % p.per_head;
+  const int64_t at = p.heads_first ? ((int64_t)b * p.heads + qh) * p.S + i
+                                   : ((int64_t)b * p.S + i) * p.heads + qh;
+  Pack<T, 4> out;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    out.v[j] = from_f32<T>(v[j] * over);
+  *(Pack<T, 4> *)((T *)p.y + at * D + 4 * d) = out;
+}
+
+// A block a row / threads a row: 16384 rows of 128 in 8 parts 70 / 53 us with the
+// attention itself, 32768 of 64 in 2 parts 87 / 49; 128 rows in 16 parts 21 / 23, 32
+// in 64 parts 41 / 51.
+template <typename T>
+hipError_t join_parts(hipStream_t st, const Arguments &p, int D, int tile_rows) {
+  const int64_t rows = (int64_t)p.B * p.c.H * p.groups * tile_rows;
+  if (p.splits <= 8) {
+    const int each = 256 / (D / 4);
+    k_cache_join_rows<T><<<dim3((unsigned)((rows + each - 1) / each)), 256, 0, st>>>(p, D, tile_rows);
+  } else {
+    k_cache_join<T><<<dim3((unsigned)rows), 256, 0, st>>>(p, D, tile_rows);
+  }
+  return hipGetLastError();
+}
+
 // How rows are dealt: tiles of 16 a wave, or of 16 / G where that takes one tile
 // (D = 64, 128, 256) or two (64, 128); or bf16's 128 rows a block, once there are
 // as many (128 rows a head, tiles / blocks: 4096 keys 31 / 27 us, 1100 keys 39 / 33;
@@ -1310,17 +1370,14 @@ hipError_t attend(hipStream_t st, const Arguments &p) {
   const int64_t units = (int64_t)p.B * p.c.H * p.groups;
   kernel<<<dim3((unsigned)(units * p.splits)), kWaves * 64, kLds, st>>>(p);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.splits > 1) {
-    k_cache_join<T><<<dim3((unsigned)(units * RT * kRows)), 256, 0, st>>>(
-        p, 32 * G, RT * kRows);
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && p.splits > 1)
+    e = join_parts<T>(st, p, 32 * G, RT * kRows);
   return e;
 }
 
 template <int G> hipError_t attend_prompt(hipStream_t st, const Arguments &p) {
-  // (keys, values and marks; then 128 rows of 64 G + 16 bytes)
-  constexpr int kLds = 8192 * G + 2048;
+  // (keys, values and marks; then 16 rows a wave of 128 G + 16 bytes)
+  constexpr int kLds = 8192 * G + 1024;
   auto *const kernel = k_cache_prompt<G>;
   if (kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute((const void *)kernel,
@@ -1331,11 +1388,8 @@ template <int G> hipError_t attend_prompt(hipStream_t st, const Arguments &p) {
   const int64_t units = (int64_t)p.B * p.c.H * p.groups;
   kernel<<<dim3((unsigned)(units * p.splits)), 256, kLds, st>>>(p);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.splits > 1) {
-    k_cache_join<__bf16><<<dim3((unsigned)(units * kPromptRows)), 256, 0, st>>>(
-        p, 32 * G, kPromptRows);
-    e = hipGetLastError();
-  }
+  if (e == hipSuccess && p.splits > 1)
+    e = join_parts<__bf16>(st, p, 32 * G, kPromptRows);
   return e;
 }
 
@@ -1420,16 +1474,19 @@ hipError_t launch_cache_append(hipStream_t s, const Append4 &a) {
 }
 
 // Parts of the keys, so that a few rows fill the GPU: two blocks a CU, which is
-// what its registers hold, of 128 keys at least.  (How many keys there are, only
+// what its registers hold (one of many rows of 256), of 128 keys at least, or 256 for
+// many rows (4 x 8 heads of 128 rows, 1100 keys, 128 / 256: 33 / 26 us).  (How many keys there are, only
 // the GPU knows: a block takes its share of what its rows see.)  131072 keys, 8
 // heads of 128, in parts for 256 / 512 / 768 / 1024 / 2048 blocks: 42 / 44 / 48 /
 // 53 / 64 us; 32 sequences of 2000 - 4000 keys 38 / 37 / 43 / 44 / 58.
 int attention_splits(const Attention4 &a) {
   const int64_t units = a.B * a.c.H * row_groups(a);
   const int64_t capacity = a.c.table ? a.c.table_pages * a.c.page_size : a.c.page_size;
-  int64_t n = 512 / (units > 0 ? units : 1);
-  if (n > (capacity + 127) / 128)
-    n = (capacity + 127) / 128;
+  const bool prompt = shape_of(a).form == Shape::kPrompt;
+  const int64_t least = prompt ? 256 : 128; // keys of a part
+  int64_t n = (prompt && a.c.D > 128 ? 256 : 512) / (units > 0 ? units : 1);
+  if (n > (capacity + least - 1) / least)
+    n = (capacity + least - 1) / least;
   return (int)(n < 1 ? 1 : n < 256 ? n : 256);
 }
 size_t attention_parts_bytes(const Attention4 &a) {
