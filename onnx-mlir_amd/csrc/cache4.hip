@@ -29,14 +29,14 @@ struct Place {
 };
 __device__ __forceinline__ Place place_of(const Cache4 &c, int64_t b, int h, int64_t key) {
   int64_t page = b, slot = key;
-  bool known = key >= 0;
-  if (c.table) {
-    const int64_t at = key / c.page_size;
-    known = known && at < c.table_pages;
-    page = known ? c.table[b * c.table_pages + at] : -1;
-    slot = key - at * c.page_size;
+  // (a sequence's pages hold 2^30 tokens at most)
+  bool known = key >= 0 && key < (c.table ? c.table_pages * c.page_size : c.page_size);
+  if (c.table && known) {
+    const unsigned at = (unsigned)key / (unsigned)c.page_size;
+    page = c.table[b * c.table_pages + at];
+    slot = (unsigned)key - at * (unsigned)c.page_size;
   }
-  known = known && page >= 0 && page < c.pages && slot < c.page_size;
+  known = known && page >= 0 && page < c.pages;
   if (!known)
     page = slot = 0;
   return {(page * c.H + h) * c.page_size + slot, (int)(c.page_size - 1 - slot), known};
@@ -58,20 +58,12 @@ __global__ __launch_bounds__(256) void k_cache_append(const Append4 p) {
   const bool value = id >= rows;
   if (value)
     id -= rows;
-  // rows in the order of k and v
-  int64_t b, i;
-  int h;
-  if (p.heads_first) {
-    const int64_t bh = id / p.S;
-    i = id - bh * p.S;
-    b = bh / p.c.H;
-    h = (int)(bh - b * p.c.H);
-  } else {
-    const int64_t t = id / p.c.H;
-    h = (int)(id - t * p.c.H);
-    b = t / p.S;
-    i = t - b * p.S;
-  }
+  // rows in the order of k and v (there are fewer than 2^31: each has 64 elements)
+  const unsigned row = (unsigned)id, S = (unsigned)p.S, H = (unsigned)p.c.H;
+  const unsigned outer = row / (p.heads_first ? S : H), inner = row - outer * (p.heads_first ? S : H);
+  const unsigned b = outer / (p.heads_first ? H : S), mid = outer - b * (p.heads_first ? H : S);
+  const int64_t i = p.heads_first ? inner : mid;
+  const int h = (int)(p.heads_first ? mid : inner);
   if (p.c.counts && i >= p.c.counts[b])
     return;
   const Place at = place_of(p.c, b, h, (int64_t)p.c.past[b] + i);
@@ -733,11 +725,12 @@ __device__ __forceinline__ unsigned high_halves(unsigned a, unsigned b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302);
 }
 // Codes in bits 0 .. 3 (LOW) or 4 .. 7 of the halves of w, as f16: 1024 + code
-// and 1024 + 16 code have the bits 0x6400 | code.
-template <bool LOW> __device__ __forceinline__ v2h codes_of(unsigned w) {
+// and 1024 + 16 code have the bits `ones` (0x6400) | code.  It comes in a register:
+// an instruction takes one constant, and so `and` and `or` are one.
+template <bool LOW> __device__ __forceinline__ v2h codes_of(unsigned w, unsigned ones) {
   if (LOW)
-    return halves_of((w & 0x000F000Fu) | 0x64006400u) - v2h{1024, 1024};
-  return __builtin_elementwise_fma(halves_of((w & 0x00F000F0u) | 0x64006400u),
+    return halves_of((w & 0x000F000Fu) | ones) - v2h{1024, 1024};
+  return __builtin_elementwise_fma(halves_of((w & 0x00F000F0u) | ones),
       v2h{0.0625f16, 0.0625f16}, v2h{-64, -64});
 }
 __device__ __forceinline__ v2h within(v2h x) { // NaN stays
@@ -925,6 +918,8 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
     }
   };
 
+  unsigned ones = 0x64006400u;
+  asm("" : "+v"(ones));
   // careful: some scale or lowest value is not finite, or what they give too large.
   auto make_keys = [&](auto careful) {
     v2h s[G], m[G]; // of the groups of bytes x, x + 2
@@ -937,10 +932,10 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
     for (int f = 0; f < G; ++f) {
       const unsigned w = raw.k[f];
       const int x = 4 * f % G, x1 = (4 * f + 1) % G;
-      v2h v[4] = {__builtin_elementwise_fma(codes_of<true>(w), s[x], m[x]),
-          __builtin_elementwise_fma(codes_of<true>(w >> 8), s[x1], m[x1]),
-          __builtin_elementwise_fma(codes_of<false>(w), s[x], m[x]),
-          __builtin_elementwise_fma(codes_of<false>(w >> 8), s[x1], m[x1])};
+      v2h v[4] = {__builtin_elementwise_fma(codes_of<true>(w, ones), s[x], m[x]),
+          __builtin_elementwise_fma(codes_of<true>(w >> 8, ones), s[x1], m[x1]),
+          __builtin_elementwise_fma(codes_of<false>(w, ones), s[x], m[x]),
+          __builtin_elementwise_fma(codes_of<false>(w >> 8, ones), s[x1], m[x1])};
       if (careful.value) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -984,8 +979,8 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const unsigned at = w[y / 2] >> (8 * (y % 2));
-          v[2 * y][i] = __builtin_elementwise_fma(codes_of<true>(at), s[i][y % SG], m[i][y % SG]);
-          v[2 * y + 1][i] = __builtin_elementwise_fma(codes_of<false>(at), s[i][y % SG], m[i][y % SG]);
+          v[2 * y][i] = __builtin_elementwise_fma(codes_of<true>(at, ones), s[i][y % SG], m[i][y % SG]);
+          v[2 * y + 1][i] = __builtin_elementwise_fma(codes_of<false>(at, ones), s[i][y % SG], m[i][y % SG]);
           if (careful.value)
             v[2 * y][i] = within(v[2 * y][i]), v[2 * y + 1][i] = within(v[2 * y + 1][i]);
         }
@@ -1049,6 +1044,14 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
         for (int r = 0; r < 2; ++r)
           s[r][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[r][f], s[r][u], 0, 0, 0);
       }
+    }
+    // Four fragments on their way (512 rows of 4 heads 50 us, 256 elements 141; with two,
+    // as they would be, 53 and 153).
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0); // LDS reads
+#pragma unroll
+    for (int i = 0; i < 4 * G; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0); // matrix instructions
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
     if (masked) {
 #pragma unroll
