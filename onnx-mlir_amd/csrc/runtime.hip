@@ -2371,8 +2371,11 @@ struct CacheViews {
           (long long)(D / kCacheGroup));
       return false;
     }
-    if (pages > kMostOfOne || H > kMostOfOne || page_size > kMostOfOne) {
-      fail(EINVAL, "%s: the cache's dimensions are too large", op);
+    // (kernels count its rows in 32 bits)
+    if (pages > kMostOfOne || H > kMostOfOne || page_size > kMostOfOne ||
+        (H > 0 && page_size > 0 &&
+            (page_size > 2 * kMostBlocks / H || pages > 2 * kMostBlocks / (H * page_size)))) {
+      fail(EINVAL, "%s: the cache has 2^32 rows or more", op);
       return false;
     }
     return true;
@@ -2471,7 +2474,20 @@ struct CacheViews {
     c.table_pages = table_pages;
     c.H = (int)H;
     c.D = (int)D;
+    on_pieces(call, c.k_codes, "k_codes");
+    on_pieces(call, c.k_scales, "k_scales");
+    on_pieces(call, c.v_codes, "v_codes");
+    on_pieces(call, c.v_scales, "v_scales");
     return c;
+  }
+
+  // Rows are read and written in pieces of 16 bytes (a row of D elements has a whole
+  // number of them, so what starts on one stays on them).
+  static void on_pieces(Call &call, const void *p, const char *name) {
+    if (!call.ok || ((uintptr_t)p & 15) == 0)
+      return;
+    fail(EINVAL, "%s: %s must start at a multiple of 16 bytes", call.op, name);
+    call.ok = false;
   }
 };
 
@@ -2699,6 +2715,8 @@ void om_mi355x_CacheAppend4(OMTensor *k_codes, OMTensor *k_scales,
   a.c = cache.on_gpu(call, /*written=*/true);
   a.k = call.in(k);
   a.v = call.in(v);
+  cache.on_pieces(call, a.k, "k");
+  cache.on_pieces(call, a.v, "v");
   a.B = h.B;
   a.S = h.S;
   a.heads_first = h.heads_first;
@@ -2770,6 +2788,8 @@ void om_mi355x_CacheAttention4(OMTensor *y_t, const OMTensor *q_t,
   a.y = counts ? call.inout(y) : call.out(y);
   a.q = call.in(q);
   a.c = cache.on_gpu(call, /*written=*/false);
+  cache.on_pieces(call, a.y, "y");
+  cache.on_pieces(call, a.q, "q");
   a.starts = starts_t ? (const int32_t *)call.in(starts) : nullptr;
   a.scale = scale_t ? (const float *)call.in(scale) : nullptr;
   a.splits = 1;

@@ -48,6 +48,15 @@ def test_matmul_blocks_refuses(om):
     refused(om, "activation 5 is not", lambda: product(activation=5))
 
 
+def test_a_product_of_too_many_elements_is_refused(om):
+    """Offsets within a tile's rows are counted in 32 bits (nothing is read)."""
+    K = 2 ** 22 + 128
+    a, b = (om.DeviceArray.wrap(4096, (n, K), om.float8_e4m3fn) for n in (1, 128))
+    sa, sb = (om.DeviceArray.wrap(4096, (1, K // 128), np.dtype(np.float32)) for _ in range(2))
+    y = om.DeviceArray.wrap(4096, (1, 128), np.dtype(np.float32))
+    refused(om, "too large|2\\^22", lambda: om.MatMulBlocks(a, sa, b, sb, out=y))
+
+
 def test_rotary_refuses(om):
     R = om.RotaryEmbedding
     x, t, p = f32(2, 3, 5, 64), f32(10, 32), np.zeros((2, 5), np.int64)
@@ -111,6 +120,18 @@ def test_cache_attention_refuses(om):
     refused(om, "past\\[0\\] is 16", lambda: A(q, c, i32(16, 0)))
     refused(om, "page_table\\[0, 0\\] is 9", lambda: A(q, c, past, np.array([[9], [0]], np.int32)))
     refused(om, "the cache has no room", lambda: A(q, om.Cache4(2, 2, 0, 64), i32(0, 0), counts=i32(0, 0)))
+
+
+def test_a_cache_of_too_many_rows_is_refused(om):
+    """Rows are counted in 32 bits (nothing is allocated, and nothing read)."""
+    c = om.Cache4(1, 1, 16, 64)
+    shape = (2 ** 20, 64, 64)
+    c.k_codes, c.v_codes = (om.DeviceArray.wrap(4096, shape + (32,), np.dtype(np.uint8)) for _ in range(2))
+    c.k_scales, c.v_scales = (om.DeviceArray.wrap(4096, shape + (2, 2), np.dtype(np.float16)) for _ in range(2))
+    k = om.DeviceArray.wrap(4096, (1, 64, 1, 64), np.dtype(np.float32))
+    past = om.DeviceArray.wrap(4096, (1,), np.dtype(np.int32))
+    refused(om, "2\\^32 rows", lambda: om.CacheAppend4(c, k, k, past))
+    refused(om, "2\\^32 rows", lambda: om.CacheAttention4(k, c, past, out=k))
 
 
 def test_types_that_numpy_lacks_keep_their_bits(om):

@@ -502,6 +502,54 @@ def test_attention(om, case, heads_first, dtype):
         assert np.array_equal(om.to_float32(again), got)
 
 
+def test_nothing_to_do(om):
+    """No rows, no columns, no tokens, no sequences."""
+    f8 = lambda *shape: np.zeros(shape, om.float8_e4m3fn)
+    one = lambda *shape: np.ones(shape, np.float32)
+    assert back(om, om.MatMulBlocks(on(om, f8(0, 128)), on(om, one(0, 1)), on(om, f8(5, 128)), on(om, one(1, 1)))).shape == (0, 5)
+    assert back(om, om.MatMulBlocks(on(om, f8(3, 128)), on(om, one(3, 1)), on(om, f8(0, 128)), on(om, one(0, 1)))).shape == (3, 0)
+    tables = on(om, one(4, 32))
+    assert back(om, om.RotaryEmbedding(on(om, one(2, 3, 0, 64)), tables, tables, on(om, np.zeros((2, 0), np.int64)))).size == 0
+    c = to_gpu(om, random_cache(om, np.random.default_rng(0), 2, 3, 16, 64))
+    kept = [bits(t.numpy()) for t in c.tensors]
+    past = on(om, np.zeros(2, np.int32))
+    om.CacheAppend4(c, on(om, one(2, 3, 0, 64)), on(om, one(2, 3, 0, 64)), past)
+    assert all(np.array_equal(bits(t.numpy()), k) for t, k in zip(c.tensors, kept))
+    assert back(om, om.CacheAttention4(on(om, one(2, 6, 0, 64)), c, past)).size == 0
+
+
+def test_cache_tensors_start_on_whole_pieces(om):
+    """What starts between two pieces of 16 bytes is refused, before any launch."""
+    d = np.dtype(np.float32)
+    room = om.DeviceArray.from_numpy(np.zeros(1 << 14, np.float32))
+    c = to_gpu(om, om.Cache4(1, 2, 16, 64))
+    whole = om.DeviceArray.wrap(room.ptr, (1, 2, 3, 64), d, owner=room)
+    odd = om.DeviceArray.wrap(room.ptr + 4, (1, 2, 3, 64), d, owner=room)
+    past = on(om, np.zeros(1, np.int32))
+    with pytest.raises(om.RuntimeError_, match="k must start at a multiple of 16 bytes"):
+        om.CacheAppend4(c, odd, whole, past)
+    with pytest.raises(om.RuntimeError_, match="q must start at"):
+        om.CacheAttention4(odd, c, past, out=whole)
+    with pytest.raises(om.RuntimeError_, match="y must start at"):
+        om.CacheAttention4(whole, c, past, out=odd)
+    c.v_scales = om.DeviceArray.wrap(room.ptr + 2, (1, 2, 16, 2, 2), np.dtype(np.float16), owner=room)
+    with pytest.raises(om.RuntimeError_, match="v_scales must start at"):
+        om.CacheAttention4(whole, c, past)
+
+
+@pytest.mark.parametrize("S", [1, 3, 140])
+def test_attention_in_place(om, S):
+    """y may be q, in one piece and in parts."""
+    rng = np.random.default_rng(S)
+    c = to_gpu(om, random_cache(om, rng, 1, 2, 1200, 128))
+    q = om.from_float32(rng.standard_normal((1, 4, S, 128)), om.bfloat16)
+    past = on(om, np.array([1000], np.int32))
+    want = bits(om.CacheAttention4(on(om, q), c, past).numpy())
+    y = on(om, q)
+    om.CacheAttention4(y, c, past, out=y)
+    assert np.array_equal(bits(y.numpy()), want)
+
+
 def test_attention_nan_of_one_sequence_stays_there(om):
     """NaN in a key that a row sees reaches that row, and not the row before it."""
     rng = np.random.default_rng(0)
