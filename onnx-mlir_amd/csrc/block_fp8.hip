@@ -523,14 +523,16 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams
 
   // Scales, one for each row and one for 128 columns, come four steps at a time, 16
   // bytes a row, 64 rows a wave: waves 0 .. BM / 64 - 1 those of the rows, the next
-  // the columns', the others nothing that is read.  A CU has some 64 requests to
+  // the columns'.  A CU has some 64 requests to
   // L2 on their way, each a line at most, and a scale by itself is one: a step's
   // 256 + 256 rows are 512, their scales one by one were 260 more (256 x 256 tiles,
   // 8192x8192x8192 530 us; every wave fetching its own 16 rows' 1170).
   constexpr int WAVES = WM * WN, NB = (BN + 2 * kBlock - 2) / kBlock; // columns' blocks
-  constexpr int SET = WAVES * 256; // floats of four steps' scales
+  constexpr int SET = (BM / 64 + 1) * 256; // floats of four steps' scales
+  // (of the waves that fetch some, so that a CU holds three blocks of 64 x 128: 520 of
+  // them, 4099 x 777 x 1001 in f32, 24.4 us, with two 27.4)
   static_assert(BM % 64 == 0 && WAVES > BM / 64 && NB <= 64, "a wave for the columns' scales");
-  float *const scales = (float *)(sm + STAGES * STAGE); // [2][WAVES][64][4]
+  float *const scales = (float *)(sm + STAGES * STAGE); // [2][BM / 64 + 1][64][4]
   const float *scale0 = p.a_scale + (int64_t)m0 * p.kblocks;
   int scale_at;
   unsigned scale_bytes; // from scale0 on
@@ -550,7 +552,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams
   }
   scale_bytes = __builtin_amdgcn_readfirstlane(scale_bytes);
   auto scales_of = [&](int kb, int set) { // (of blocks kb .. kb + 3)
-    copy16(scale0, scales + set * SET + wave * 256, scale_at, kb * 4, scale_bytes);
+    if (wave <= BM / 64)
+      copy16(scale0, scales + set * SET + wave * 256, scale_at, kb * 4, scale_bytes);
   };
 
   float total[TM][TN][4];
@@ -763,7 +766,7 @@ __global__ __launch_bounds__(256) void k_join_parts(const GemmParams p) {
 }
 
 // Rows of up to two matrices copied to a pitch of whole 16-byte chunks, zeros
-// behind them.
+// behind them, a wave a row.
 struct AlignRows {
   const uint8_t *from[2];
   uint8_t *to[2];
@@ -771,26 +774,27 @@ struct AlignRows {
   int K, pitch;
 };
 __global__ __launch_bounds__(256) void k_align_rows(const AlignRows p) {
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int chunks = p.pitch / 16;
-  int64_t row = id / chunks;
-  const int k = (int)(id - row * chunks) * 16;
+  int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int which = row >= p.rows[0];
   row -= which ? p.rows[0] : 0;
   if (row >= p.rows[which])
     return;
-  const uint8_t *const x = p.from[which] + row * p.K + k;
-  v4u w = {0, 0, 0, 0};
-  if (k + 16 <= p.K) {
-    typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
-    w = *(const v4u_any *)x;
-  } else {
+  const uint8_t *const x = p.from[which] + row * p.K;
+  uint8_t *const y = p.to[which] + row * p.pitch;
+#pragma unroll 2
+  for (int k = threadIdx.x % 64 * 16; k < p.pitch; k += 64 * 16) {
+    v4u w = {0, 0, 0, 0};
+    if (k + 16 <= p.K) {
+      typedef unsigned v4u_any __attribute__((ext_vector_type(4), aligned(1)));
+      w = *(const v4u_any *)(x + k);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (k + i < p.K)
-        w[i / 4] |= (unsigned)x[i] << (8 * (i % 4));
+      for (int i = 0; i < 16; ++i)
+        if (k + i < p.K)
+          w[i / 4] |= (unsigned)x[k + i] << (8 * (i % 4));
+    }
+    *(v4u *)(y + k) = w;
   }
-  *(v4u *)(p.to[which] + row * p.pitch + k) = w;
 }
 
 // Rows that the kernel for few of them takes: 16, and 32 of small products, where a
@@ -896,7 +900,7 @@ const char *tile_name(int bm, int bn, bool parts) {
 template <typename T, int BM, int BN, int WM, int WN, int STAGES>
 hipError_t tile(hipStream_t st, const GemmParams &p) {
   constexpr bool kExact = sizeof(T) == 4;
-  constexpr int kLds = STAGES * (BM + BN) * kBlock + 2 * WM * WN * 1024;
+  constexpr int kLds = STAGES * (BM + BN) * kBlock + 2 * (BM / 64 + 1) * 1024;
   static_assert(kLds <= 160 * 1024, "LDS");
   auto *const kernel = k_block_tile<T, BM, BN, WM, WN, STAGES, kExact>;
   if (kLds > 65536) {
@@ -1008,8 +1012,8 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
     if (n) {
       copies.K = (int)g.K;
       copies.pitch = pitch;
-      const int64_t chunks = (copies.rows[0] + copies.rows[1]) * (pitch / 16);
-      k_align_rows<<<dim3((unsigned)((chunks + 255) / 256)), 256, 0, s>>>(copies);
+      const int64_t blocks = (copies.rows[0] + copies.rows[1] + 3) / 4;
+      k_align_rows<<<dim3((unsigned)blocks), 256, 0, s>>>(copies);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess)
         return e;
