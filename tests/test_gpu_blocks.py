@@ -550,6 +550,23 @@ def test_attention_in_place(om, S):
     assert np.array_equal(bits(y.numpy()), want)
 
 
+@pytest.mark.parametrize("dtype,S", [("f32", 5), ("bf16", 5), ("bf16", 140)])
+def test_attention_of_positions_that_the_cache_does_not_hold(om, dtype, S):
+    """past in GPU memory is not checked: tokens in front of the first one see nothing,
+    those behind the last one all that there is; more counts than rows are all rows."""
+    rng = np.random.default_rng(S)
+    size = 300
+    c = to_gpu(om, random_cache(om, rng, 2, 1, size, 64))
+    q = om.from_float32(rng.standard_normal((2, 1, S, 64)), dt(om, dtype))
+    past = on(om, np.array([-3, 2 ** 31 - 1], np.int32))
+    got = back(om, om.CacheAttention4(on(om, q), c, past, counts=on(om, np.array([S + 7, 2 ** 31 - 1], np.int32))))
+    assert not got[0, 0, :3].any()
+    late = on(om, np.array([-3, size - S], np.int32))
+    assert equal(got[0], back(om, om.CacheAttention4(on(om, q), c, late))[0])
+    assert np.isfinite(got).all() and got[0, 0, 3:].any()
+    assert equal(got[1], back(om, om.CacheAttention4(on(om, q), c, late, causal=0))[1])
+
+
 def test_attention_nan_of_one_sequence_stays_there(om):
     """NaN in a key that a row sees reaches that row, and not the row before it."""
     rng = np.random.default_rng(0)
