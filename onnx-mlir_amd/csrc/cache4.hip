@@ -716,6 +716,11 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
 // keys 4 h .. of either 16, element 16 t + c in the order z (4 G) + j: byte z / 2 of
 // word j, z % 2 its half.  All are read as they lie, 1024 bytes after one another.
 //
+// 2048 rows on 4096 keys, 32 heads on 8 of 128, causal: 142 us, 730 TFLOP/s (534 us in
+// tiles).  Bound by vector instructions: of some 300 a wave takes for 64 keys, 130 make
+// its share of them and 32 are exponentials at a quarter of the rate; two blocks a CU
+// overlap them with 64 matrix instructions in part.
+//
 // A group of a value whose scale or lowest value is not finite must give NaN to rows
 // that see its key and nothing to others: it is made into zeros, and marked.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
