@@ -717,9 +717,10 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
 // word j, z % 2 its half.  All are read as they lie, 1024 bytes after one another.
 //
 // 2048 rows on 4096 keys, 32 heads on 8 of 128, causal: 142 us, 730 TFLOP/s (534 us in
-// tiles).  Bound by vector instructions: of some 300 a wave takes for 64 keys, 130 make
-// its share of them and 32 are exponentials at a quarter of the rate; two blocks a CU
-// overlap them with 64 matrix instructions in part.
+// tiles).  Bound by instructions: vector ones take 48 % of the clocks (of some 300 for 64
+// keys a wave, 130 make its share of them and 32 are exponentials at a quarter of the
+// rate), matrix ones 28 %, and the two blocks that a CU has registers for overlap little;
+// blocks of unequal length leave it with one for the rest.
 //
 // A group of a value whose scale or lowest value is not finite must give NaN to rows
 // that see its key and nothing to others: it is made into zeros, and marked.
@@ -1162,6 +1163,8 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
     sum[r] += __shfl_xor(sum[r], 32);
     nan[r] |= __shfl_xor(nan[r], 16);
     nan[r] |= __shfl_xor(nan[r], 32);
+    if (scale != scale && sum[r] > 0.0f) // (rows that see nothing stay 0)
+      nan[r] = ~0u;
   }
   // Element 4 h + i of tile t is z (4 G) + j.
   auto element_of = [&](int t, int i, int &g) {

@@ -550,6 +550,26 @@ def test_attention_in_place(om, S):
     assert np.array_equal(bits(y.numpy()), want)
 
 
+@pytest.mark.parametrize("dtype,S", [("f16", 1), ("f32", 40), ("bf16", 140)])
+def test_attention_of_queries_and_scales_that_are_not_finite(om, dtype, S):
+    """A query's NaN or infinity makes its own row NaN; a scale of NaN every row that
+    sees a key."""
+    rng = np.random.default_rng(S)
+    c = to_gpu(om, random_cache(om, rng, 3, 1, 200, 128))
+    x = rng.standard_normal((3, 2, S, 128)).astype(np.float32)
+    past, starts = on(om, np.full(3, 20, np.int32)), on(om, np.array([0, 0, 190], np.int32))
+    plain = back(om, om.CacheAttention4(on(om, om.from_float32(x, dt(om, dtype))), c, past, starts=starts))
+    bad = np.zeros((3, 2, S), bool)
+    bad[0, 1, 0] = bad[1, 0, S - 1] = True
+    x[0, 1, 0, 77] = np.nan
+    x[1, 0, S - 1, 5] = np.inf
+    q = on(om, om.from_float32(x, dt(om, dtype)))
+    got = back(om, om.CacheAttention4(q, c, past, starts=starts))
+    assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], plain[~bad])
+    got = back(om, om.CacheAttention4(q, c, past, starts=starts, scale=on(om, np.float32(np.nan))))
+    assert np.isnan(got[:2]).all() and not got[2].any()
+
+
 @pytest.mark.parametrize("dtype,S", [("f32", 5), ("bf16", 5), ("bf16", 140)])
 def test_attention_of_positions_that_the_cache_does_not_hold(om, dtype, S):
     """past in GPU memory is not checked: tokens in front of the first one see nothing,
