@@ -330,9 +330,17 @@ __device__ __forceinline__ void copy16(
 // instructions; sums of the waves meet in LDS in a fixed order.
 // One row, 4096 x 11008: 11.5 us (12.4 with scales asked for by every wave, 11.9
 // with the weights copied into LDS, 9.8 with neither rows of a nor scales).
-// TAIL: any K and any alignment, what lies past a row's end 0.
+// TAIL: any K and any alignment, what lies past a row's end 0; and any number of
+// rows, 16 MT a blockIdx.y, for products that have no room for aligned copies.
 template <typename T, int MT, int WAVES, int DEPTH, bool TAIL, bool STAGED>
-__global__ __launch_bounds__(WAVES * 64) void k_block_skinny(const GemmParams p) {
+__global__ __launch_bounds__(WAVES * 64) void k_block_skinny(GemmParams p) {
+  if (TAIL) {
+    const int m0 = blockIdx.y * (16 * MT);
+    p.a += (int64_t)m0 * p.lda;
+    p.a_scale += (int64_t)m0 * p.kblocks;
+    p.y = (T *)p.y + (int64_t)m0 * p.N;
+    p.M = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
+  }
   extern __shared__ float staged[]; // scales of b's columns, then of a's rows
   __shared__ v4f sums[WAVES][MT][64];
   const int lane = threadIdx.x & 63;
@@ -811,9 +819,10 @@ bool rows_aligned(const void *p, int64_t K) {
 
 template <typename T, int MT, int WAVES, int DEPTH, bool TAIL>
 hipError_t skinny_in(hipStream_t st, const GemmParams &p) {
-  const dim3 grid((unsigned)((p.N + 15) / 16)), block(WAVES * 64);
+  const int rows = p.M < 16 * MT ? p.M : 16 * MT; // of a block
+  const dim3 grid((unsigned)((p.N + 15) / 16), (unsigned)((p.M + rows - 1) / rows)), block(WAVES * 64);
   // (32 KB of scales: 16 rows of 61000 elements)
-  const int64_t floats = (int64_t)(p.M + 1) * p.kblocks;
+  const int64_t floats = (int64_t)(rows + 1) * p.kblocks;
   if (floats <= 8192)
     k_block_skinny<T, MT, WAVES, DEPTH, TAIL, true><<<grid, block, (size_t)floats * 4, st>>>(p);
   else
@@ -831,6 +840,7 @@ hipError_t skinny(hipStream_t st, const GemmParams &p) {
 
 // Tiles that a product can be dealt in.
 enum TileForm { k256x256, k256x128, k128x128, k64x128, kTileForms };
+constexpr int kUnaligned = kTileForms; // no tiles: rows that they cannot copy
 
 // Which tile, and in how many parts of K: what takes the least time by
 //   base + steps (full rounds * full + the rest of the fullest CU * lone) + rounds * round
@@ -860,7 +870,7 @@ struct TilePlan {
 };
 constexpr int kMostParts = 16;
 constexpr int64_t kMostSums = (int64_t)64 << 20; // of all parts
-TilePlan plan_tiles(const BlockGemm &g) {
+TilePlan plan_tiles(const BlockGemm &g, int most_parts = kMostParts) {
   const int64_t kblocks = (g.K + kBlock - 1) / kBlock;
   TilePlan best = {k128x128, 1};
   float least = 0.0f;
@@ -869,7 +879,7 @@ TilePlan plan_tiles(const BlockGemm &g) {
     if (!c.bm)
       continue;
     const int64_t tiles = ((g.M + c.bm - 1) / c.bm) * ((g.N + c.bn - 1) / c.bn);
-    for (int parts = 1; parts <= kMostParts; parts *= 2) {
+    for (int parts = 1; parts <= most_parts; parts *= 2) {
       if (parts > 1 && (parts > kblocks || g.M * g.N > kMostSums / parts))
         break;
       const int64_t steps = (kblocks + parts - 1) / parts;
@@ -921,10 +931,28 @@ hipError_t tile(hipStream_t st, const GemmParams &p) {
   return e;
 }
 
+// Rows where they lie, any number of them, in launches of as many as a grid has.
+template <typename T> hipError_t unaligned(hipStream_t st, GemmParams p) {
+  note_gemm_kernel("k_block_skinny (many rows)");
+  constexpr int kRows = 32 * 65535;
+  for (int left = p.M; left > 0; left -= kRows) {
+    p.M = left < kRows ? left : kRows;
+    const hipError_t e = skinny_in<T, 2, 8, 2, true>(st, p);
+    if (e != hipSuccess)
+      return e;
+    p.a += (int64_t)kRows * p.lda;
+    p.a_scale += (int64_t)kRows * p.kblocks;
+    p.y = (T *)p.y + (int64_t)kRows * p.N;
+  }
+  return hipSuccess;
+}
+
 template <typename T>
 hipError_t product(hipStream_t st, const GemmParams &p, int form) {
   if (few_rows(p.M, p.K, p.N))
     return p.M <= 16 ? skinny<T, 1>(st, p) : skinny<T, 2>(st, p);
+  if (form == kUnaligned)
+    return unaligned<T>(st, p);
   // (f32 results of larger tiles do not fit in LDS)
   if constexpr (sizeof(T) == 2) {
     switch (form) {
@@ -955,7 +983,7 @@ hipError_t launch_quantize_blocks(hipStream_t s, const void *x, FloatKind kind,
 }
 
 // The tile kernel copies 16-byte chunks of rows that start on such: others are
-// copied first.
+// copied first, or, without room for that, multiplied where they lie.
 static size_t aligned_bytes(const void *p, int64_t rows, int64_t K) {
   return rows_aligned(p, K) ? 0 : (size_t)rows * (size_t)((K + 15) / 16 * 16);
 }
@@ -963,13 +991,18 @@ static int64_t part_pitch(const BlockGemm &g) { return (g.N + 3) / 4 * 4; }
 static size_t parts_bytes(const BlockGemm &g, const TilePlan &plan) {
   return plan.parts > 1 ? (size_t)plan.parts * g.M * part_pitch(g) * sizeof(float) : 0;
 }
-size_t block_gemm_scratch(const BlockGemm &g) {
+size_t block_gemm_row_bytes(const BlockGemm &g) {
   if (few_rows(g.M, g.K, g.N))
     return 0;
-  return aligned_bytes(g.a, g.M, g.K) + aligned_bytes(g.b, g.N, g.K) + parts_bytes(g, plan_tiles(g));
+  return aligned_bytes(g.a, g.M, g.K) + aligned_bytes(g.b, g.N, g.K);
+}
+size_t block_gemm_part_bytes(const BlockGemm &g) {
+  if (few_rows(g.M, g.K, g.N) || (!g.rows && block_gemm_row_bytes(g)))
+    return 0;
+  return parts_bytes(g, plan_tiles(g));
 }
 
-hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
+hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g) {
   GemmParams p = {};
   p.a = g.a;
   p.b = g.b;
@@ -986,14 +1019,16 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch) {
   p.parts = 1;
   p.part_blocks = p.kblocks;
   TilePlan plan = {};
-  if (!few_rows(g.M, g.K, g.N)) {
-    plan = plan_tiles(g);
-    uint8_t *at = (uint8_t *)scratch;
+  if (few_rows(g.M, g.K, g.N)) {
+  } else if (!g.rows && block_gemm_row_bytes(g)) {
+    plan.form = kUnaligned;
+  } else {
+    plan = plan_tiles(g, g.parts ? kMostParts : 1);
     p.parts = plan.parts;
     p.part_blocks = (p.kblocks + plan.parts - 1) / plan.parts;
     p.part_pitch = (int)part_pitch(g);
-    p.part_sums = (float *)at;
-    at += parts_bytes(g, plan); // (a multiple of 16)
+    p.part_sums = g.parts;
+    uint8_t *at = g.rows;
     const int pitch = (int)((g.K + 15) / 16 * 16);
     AlignRows copies = {};
     int n = 0;

@@ -31,10 +31,14 @@ struct BlockGemm {
   int64_t bias_len;
   FloatKind kind; // of y
   int activation; // OM_MI355X_ACTIVATION_*
+  // Scratch, aligned to 16 bytes, without which the product is slower:
+  uint8_t *rows; // block_gemm_row_bytes(): aligned copies of rows
+  float *parts;  // block_gemm_part_bytes(): sums of parts of K
 };
-// Bytes of scratch that the product needs (0: none): aligned copies of rows.
-size_t block_gemm_scratch(const BlockGemm &g);
-hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g, void *scratch);
+// 0: none is of use.  `parts` is asked for once `rows` is known.
+size_t block_gemm_row_bytes(const BlockGemm &g);
+size_t block_gemm_part_bytes(const BlockGemm &g);
+hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g);
 
 // ---- rotary positions ------------------------------------------------------
 struct Rotary {

@@ -2604,12 +2604,13 @@ void om_mi355x_MatMulBlocks(OMTensor *y_t, const OMTensor *a_t,
     g.bias_len = bias.numel;
   }
   g.activation = (int)activation;
-  void *scratch = nullptr;
-  if (call.ok)
-    if (const size_t bytes = block_gemm_scratch(g))
-      scratch = call.temp(bytes);
-  if (call.ok)
-    call.check(launch_block_gemm(call.c.stream, g, scratch), op);
+  if (call.ok) {
+    if (const size_t bytes = block_gemm_row_bytes(g))
+      g.rows = (uint8_t *)call.scratch_for(bytes);
+    if (const size_t bytes = block_gemm_part_bytes(g))
+      g.parts = (float *)call.scratch_for(bytes);
+    call.check(launch_block_gemm(call.c.stream, g), op);
+  }
   call.finish();
 }
 
