@@ -310,8 +310,9 @@ __device__ __forceinline__ void store4(
   }
 }
 
-// 16 bytes a lane from `from` + at + k (k the same in all lanes; nothing from
-// `bytes` on) into LDS, the wave's from `to` on, one after the other.
+// 16 bytes a lane from `from` + at + k (k the same in all lanes) into LDS, the wave's
+// from `to` on, one after the other.  Nothing comes from `bytes` on where k is 0: only
+// a lane's own offset takes part in the range check.
 __device__ __forceinline__ void copy16(
     const void *from, void *to, int at, int k, unsigned bytes = 0x7FFFFFFF) {
   typedef __attribute__((address_space(3))) void *lds_ptr;
@@ -559,9 +560,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void k_block_tile(const GemmParams
     scale_bytes = bytes < 0x7FFFFFFF ? (unsigned)bytes : 0x7FFFFFFFu;
   }
   scale_bytes = __builtin_amdgcn_readfirstlane(scale_bytes);
-  auto scales_of = [&](int kb, int set) { // (of blocks kb .. kb + 3)
+  // Of blocks kb .. kb + 3; those behind a row's last are the next row's, and behind
+  // the last row's nothing is read.
+  auto scales_of = [&](int kb, int set) {
     if (wave <= BM / 64)
-      copy16(scale0, scales + set * SET + wave * 256, scale_at, kb * 4, scale_bytes);
+      copy16(scale0, scales + set * SET + wave * 256, scale_at + kb * 4, 0, scale_bytes);
   };
 
   float total[TM][TN][4];

@@ -817,3 +817,20 @@ def test_two_threads_at_once(om):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("M,K,N,dtype", [
+    (1024, 100, 128, "bf16"), (1024, 640, 300, "f32"), (1024, 520, 1024, "f16"), (1024, 1152, 4096, "bf16"), (1024, 4096, 130, "f32")])
+def test_matmul_blocks_scales_at_the_end_of_their_memory(om, M, K, N, dtype):
+    """Scales are fetched four blocks of K at a time, also where fewer are left: what
+    lies behind the last one, here another page's NaN, is neither read as one nor
+    needed.  (Tensors that fill whole pages.)"""
+    rng = np.random.default_rng(K)
+    a, sa, b, sb = operands(om, rng, M, K, N)
+    assert sa.nbytes % 4096 == 0
+    room = np.full(4096 + sb.size, np.nan, np.float32)
+    room[4096 - sb.size:4096] = sb.reshape(-1)
+    scales = om.DeviceArray.view_of(on(om, room), 4096 - sb.size, sb.shape)
+    got = om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), scales, dtype=dt(om, dtype))
+    want, size = product(om, a, sa, b, sb)
+    check_product(om, back(om, got), want, size, dtype, M, K)
