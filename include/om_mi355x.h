@@ -253,7 +253,8 @@ void om_mi355x_DynamicQuantizeBlocks(OMTensor *y, OMTensor *y_scale,
  * y: float [.., N]; a: f8e4m3fn [.., K], its leading dimensions folded into M;
  * a_scale: f32 [.., ceil(K/128)]; b: f8e4m3fn [N, K]; b_scale: f32
  * [ceil(N/128), ceil(K/128)]; bias: NULL, f32 scalar or [N]; activation as for
- * om_mi355x_MatMulIntegerDequant.  K is at most 2^22.
+ * om_mi355x_MatMulIntegerDequant.  K is at most 2^22, N 2^27 - 128, M 2^30, and
+ * there are fewer than 2^23 blocks of 128 x 128 results.
  * Where y has 16 bits and more than 16 rows, the products of a block are added
  * by matrix instructions for 8-bit operands, whose sums are off by up to 1e-4
  * of the result's magnitude, less than y's own rounding; otherwise they are

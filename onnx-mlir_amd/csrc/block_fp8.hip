@@ -186,27 +186,38 @@ __global__ __launch_bounds__(256) void k_quantize_tiles(
     scale[blockIdx.x] = s;
 }
 
+// (A launch's rows, or tiles of 128: those of the most blocks that it may have.)
 template <typename T>
 hipError_t quantize(hipStream_t st, const T *x, int64_t M, int64_t K, int rows,
     uint8_t *y, float *scale) {
   const int per_row = (int)((K + kBlock - 1) / kBlock);
   const bool wide = K % 8 == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)y & 7) == 0;
-  if (rows == 1) {
-    const int64_t blocks = M * per_row;
-    constexpr int U = 2;
-    const dim3 grid((unsigned)((blocks + 16 * U - 1) / (16 * U)));
-    if (wide)
-      k_quantize_rows<T, true, U><<<grid, 256, 0, st>>>(x, y, scale, blocks, (int)K, per_row);
-    else
-      k_quantize_rows<T, false, U><<<grid, 256, 0, st>>>(x, y, scale, blocks, (int)K, per_row);
-  } else {
-    const dim3 grid((unsigned)((M + 127) / 128 * per_row));
-    if (wide)
-      k_quantize_tiles<T, true><<<grid, 256, 0, st>>>(x, y, scale, M, (int)K, per_row);
-    else
-      k_quantize_tiles<T, false><<<grid, 256, 0, st>>>(x, y, scale, M, (int)K, per_row);
+  constexpr int U = 2;
+  const int64_t most = rows == 1 ? kMostGrid * 16 * U / per_row : kMostGrid / per_row * 128;
+  for (; M > 0; M -= most) {
+    const int64_t m = M < most ? M : most;
+    if (rows == 1) {
+      const int64_t blocks = m * per_row;
+      const dim3 grid((unsigned)((blocks + 16 * U - 1) / (16 * U)));
+      if (wide)
+        k_quantize_rows<T, true, U><<<grid, 256, 0, st>>>(x, y, scale, blocks, (int)K, per_row);
+      else
+        k_quantize_rows<T, false, U><<<grid, 256, 0, st>>>(x, y, scale, blocks, (int)K, per_row);
+    } else {
+      const dim3 grid((unsigned)((m + 127) / 128 * per_row));
+      if (wide)
+        k_quantize_tiles<T, true><<<grid, 256, 0, st>>>(x, y, scale, m, (int)K, per_row);
+      else
+        k_quantize_tiles<T, false><<<grid, 256, 0, st>>>(x, y, scale, m, (int)K, per_row);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return e;
+    x += m * K;
+    y += m * K;
+    scale += (m + rows - 1) / rows * per_row;
   }
-  return hipGetLastError();
+  return hipSuccess;
 }
 
 // ---------------------------------------------------------------------------
@@ -782,10 +793,11 @@ struct AlignRows {
   const uint8_t *from[2];
   uint8_t *to[2];
   int64_t rows[2];
+  int64_t first; // of a launch
   int K, pitch;
 };
 __global__ __launch_bounds__(256) void k_align_rows(const AlignRows p) {
-  int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  int64_t row = p.first + (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
   const int which = row >= p.rows[0];
   row -= which ? p.rows[0] : 0;
   if (row >= p.rows[which])
@@ -1050,11 +1062,13 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g) {
     if (n) {
       copies.K = (int)g.K;
       copies.pitch = pitch;
-      const int64_t blocks = (copies.rows[0] + copies.rows[1] + 3) / 4;
-      k_align_rows<<<dim3((unsigned)blocks), 256, 0, s>>>(copies);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess)
-        return e;
+      int64_t blocks = (copies.rows[0] + copies.rows[1] + 3) / 4;
+      for (copies.first = 0; blocks > 0; blocks -= kMostGrid, copies.first += 4 * kMostGrid) {
+        k_align_rows<<<dim3((unsigned)(blocks < kMostGrid ? blocks : kMostGrid)), 256, 0, s>>>(copies);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess)
+          return e;
+      }
     }
     if (p.lda == pitch && p.ldb == pitch)
       p.K = pitch; // (zeros behind the last element of both)

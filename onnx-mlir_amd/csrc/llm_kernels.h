@@ -12,6 +12,11 @@ namespace om {
 // Element types of activations; everything is computed in f32.
 enum FloatKind : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 
+// HIP counts a launch's threads in 32 bits along each axis, and takes more than that
+// for what is left of them: a launch has at most this many blocks (of up to 256
+// threads), and what needs more takes several.
+constexpr int64_t kMostGrid = (int64_t)1 << 23;
+
 // ---- e4m3 with a scale for each block --------------------------------------
 constexpr int kBlock = 128; // elements of a row under one scale
 

@@ -21,6 +21,7 @@ struct RotaryArgs {
   const float *cos, *sin;
   const int64_t *positions;
   int64_t S, table_rows, rows; // rows: B * S * H
+  int64_t first;               // row of a launch
   int H, D, half;              // half: rot / 2
   int units;                   // threads a row takes
   bool heads_first;
@@ -31,8 +32,9 @@ struct RotaryArgs {
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void k_rotary(const RotaryArgs p) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / p.units;
+  int64_t row = id / p.units;
   const int u = (int)(id - row * p.units);
+  row += p.first;
   if (row >= p.rows)
     return;
   int64_t token; // b * S + s
@@ -107,23 +109,29 @@ template <typename T>
 hipError_t launch(hipStream_t st, const Rotary &r) {
   constexpr int V = 16 / (int)sizeof(T);
   RotaryArgs p = {r.x, r.y, r.cos, r.sin, r.positions, r.S, r.table_rows,
-      r.B * r.S * r.H, (int)r.H, r.D, r.rot / 2, 0, r.heads_first};
+      r.B * r.S * r.H, 0, (int)r.H, r.D, r.rot / 2, 0, r.heads_first};
   // 16-byte pieces: the halves of a head, what passes through, and every row.
   const auto aligned = [](const void *q) { return ((uintptr_t)q & 15) == 0; };
   const bool wide = p.half % V == 0 && (r.D - r.rot) % (2 * V) == 0 &&
                     aligned(r.x) && aligned(r.y) && aligned(r.cos) && aligned(r.sin);
   p.units = wide ? r.D / 2 / V : (r.D + 1) / 2;
-  const int64_t blocks = (p.rows * p.units + 255) / 256;
-  const dim3 grid((unsigned)blocks), block(256);
-  if (wide && r.interleaved)
-    k_rotary<T, V, true><<<grid, block, 0, st>>>(p);
-  else if (wide)
-    k_rotary<T, V, false><<<grid, block, 0, st>>>(p);
-  else if (r.interleaved)
-    k_rotary<T, 1, true><<<grid, block, 0, st>>>(p);
-  else
-    k_rotary<T, 1, false><<<grid, block, 0, st>>>(p);
-  return hipGetLastError();
+  const int64_t most = kMostGrid * 256 / p.units; // rows of a launch
+  for (; p.first < p.rows; p.first += most) {
+    const int64_t rows = p.rows - p.first < most ? p.rows - p.first : most;
+    const dim3 grid((unsigned)((rows * p.units + 255) / 256)), block(256);
+    if (wide && r.interleaved)
+      k_rotary<T, V, true><<<grid, block, 0, st>>>(p);
+    else if (wide)
+      k_rotary<T, V, false><<<grid, block, 0, st>>>(p);
+    else if (r.interleaved)
+      k_rotary<T, 1, true><<<grid, block, 0, st>>>(p);
+    else
+      k_rotary<T, 1, false><<<grid, block, 0, st>>>(p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return e;
+  }
+  return hipSuccess;
 }
 
 } // namespace

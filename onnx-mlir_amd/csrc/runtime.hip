@@ -2583,9 +2583,10 @@ void om_mi355x_MatMulBlocks(OMTensor *y_t, const OMTensor *a_t,
   bool relu, gelu;
   if (!activation_ok(activation, op, relu, gelu))
     return;
-  // (rows of a tile are addressed by 31-bit offsets)
-  if (g.M > kMostOfOne || g.N > kMostOfOne || g.K > ((int64_t)1 << 22) ||
-      blocks_of(g.M) * blocks_of(g.N) > kMostBlocks / 32) {
+  // (rows of a tile are addressed by 31-bit offsets; 16 columns of few rows, or 128 x
+  // 128 results in tiles, take 512 threads, of which a launch has fewer than 2^32)
+  if (g.M > kMostOfOne || g.N > ((int64_t)1 << 27) - kBlock || g.K > ((int64_t)1 << 22) ||
+      blocks_of(g.M) * blocks_of(g.N) >= (int64_t)1 << 23) {
     fail(EINVAL, "%s: the product is too large", op);
     return;
   }

@@ -57,6 +57,15 @@ def test_a_product_of_too_many_elements_is_refused(om):
     refused(om, "too large|2\\^22", lambda: om.MatMulBlocks(a, sa, b, sb, out=y))
 
 
+@pytest.mark.parametrize("M,N", [(1, 2 ** 27 - 127), (2 ** 30 + 1, 1), (2 ** 30, 1), (2 ** 18, 2 ** 19)])
+def test_a_product_of_too_many_results_is_refused(om, M, N):
+    """A launch has fewer than 2^32 threads (nothing is read)."""
+    wrap = lambda shape, dtype: om.DeviceArray.wrap(4096, shape, np.dtype(dtype))
+    a, b = wrap((M, 128), om.float8_e4m3fn), wrap((N, 128), om.float8_e4m3fn)
+    sa, sb = wrap((M, 1), np.float32), wrap((-(-N // 128), 1), np.float32)
+    refused(om, "too large", lambda: om.MatMulBlocks(a, sa, b, sb, out=wrap((M, N), np.float32)))
+
+
 def test_rotary_refuses(om):
     R = om.RotaryEmbedding
     x, t, p = f32(2, 3, 5, 64), f32(10, 32), np.zeros((2, 5), np.int64)

@@ -834,3 +834,71 @@ def test_matmul_blocks_scales_at_the_end_of_their_memory(om, M, K, N, dtype):
     got = om.MatMulBlocks(on(om, a), on(om, sa), on(om, b), scales, dtype=dt(om, dtype))
     want, size = product(om, a, sa, b, sb)
     check_product(om, back(om, got), want, size, dtype, M, K)
+
+
+# Launches of 2^32 threads: HIP counts a grid's in 32 bits.
+def on_torch(om, t, dtype):
+    return om.DeviceArray.wrap(t.data_ptr(), tuple(t.shape), dtype, owner=t)
+
+
+def all_are(t, value):
+    """(By itself: an assertion that shows such a tensor takes minutes.)"""
+    return bool((t == value).all())
+
+
+@pytest.mark.parametrize("M,rows,dtype", [(2 ** 29 + 64, 1, "f32"), (2 ** 31 + 192, 128, "f16")])
+def test_quantize_blocks_of_many_rows(om, M, rows, dtype):
+    torch = pytest.importorskip("torch")
+    x = torch.ones((M, 1), dtype={"f32": torch.float32, "f16": torch.float16}[dtype], device="cuda")
+    x[-64:] = -3.0
+    y = torch.zeros((M, 1), dtype=torch.uint8, device="cuda")
+    s = torch.zeros((-(-M // rows), 1), device="cuda")
+    torch.cuda.synchronize()
+    om.DynamicQuantizeBlocks(on_torch(om, x, dt(om, dtype)), rows, out=(on_torch(om, y, om.float8_e4m3fn), on_torch(om, s, np.dtype(np.float32))))
+    om.synchronize()
+    assert all_are(y[:-64], 0x7E) and all_are(y[-64:], 0xFE)
+    of = 64 // rows or 1  # (the last 64 rows are blocks of their own)
+    assert all_are(s[:-of], float(np.float32(1) / np.float32(448))) and all_are(s[-of:], float(np.float32(3) / np.float32(448)))
+
+
+def test_matmul_blocks_of_many_rows(om):
+    torch = pytest.importorskip("torch")
+    M, K = 2 ** 26 + 64, 17
+    a = torch.full((M, K), 0x38, dtype=torch.uint8, device="cuda")
+    a[-70:] = 0x40
+    sa = torch.ones((M, 1), device="cuda")
+    y = torch.zeros((M, 1), device="cuda")
+    torch.cuda.synchronize()
+    b, sb = np.full((1, K), 0x38, np.uint8).view(om.float8_e4m3fn), np.ones((1, 1), np.float32)
+    f32 = np.dtype(np.float32)
+    om.MatMulBlocks(on_torch(om, a, om.float8_e4m3fn), on_torch(om, sa, f32), on(om, b), on(om, sb), out=on_torch(om, y, f32))
+    om.synchronize()
+    assert all_are(y[:-70], K) and all_are(y[-70:], 2 * K)
+
+
+def test_rotary_of_many_rows(om):
+    torch = pytest.importorskip("torch")
+    S, H = 2 ** 16, 2 ** 16 + 1
+    x = torch.ones((1, S, 2 * H), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    d = on_torch(om, x, om.bfloat16)
+    om.RotaryEmbedding(d, on(om, np.zeros((1, 1), np.float32)), on(om, np.ones((1, 1), np.float32)),
+                       on(om, np.zeros((1, S), np.int64)), num_heads=H, out=d)
+    om.synchronize()
+    assert all_are(x[..., 0::2], -1) and all_are(x[..., 1::2], 1)
+
+
+def test_append_many_rows(om):
+    """The last 16 rows of 2^27 and more have places."""
+    torch = pytest.importorskip("torch")
+    S = 2 ** 27 + 64
+    k = torch.empty((1, 1, S, 64), dtype=torch.bfloat16, device="cuda")
+    rng = np.random.default_rng(0)
+    rows = om.from_float32(rng.standard_normal((16, 64)), om.bfloat16)
+    k[0, 0, -16:] = torch.from_numpy(om.to_float32(rows)).to(torch.bfloat16).cuda()
+    torch.cuda.synchronize()
+    c = to_gpu(om, om.Cache4(1, 1, 16, 64))
+    d = on_torch(om, k, om.bfloat16)
+    om.CacheAppend4(c, d, d, on(om, np.array([16 - S], np.int32)))
+    qc, qs = ref.quantize4(om.to_float32(rows))
+    assert all(np.array_equal(g.numpy()[0, 0], w) for g, w in zip(c.tensors, (qc, qs, qc, qs)))
