@@ -141,6 +141,10 @@ __global__ __launch_bounds__(256) void k_cache_append(const Append4 p, int64_t f
 // for group g, of whose elements alone the results are kept.  The matrix
 // instructions are as many, the vector ones, which bound the kernel, less than
 // half: a lane scales and splits 8 weights for 32 keys, not 8 G.
+//
+// An infinity in a query, or as the scale, makes every score infinite or NaN, and so
+// each row that sees a key NaN: it is taken as NaN, for scores of -inf alone would
+// look like a row that sees none.
 struct Arguments {
   Cache4 c;
   const void *q;
@@ -153,6 +157,8 @@ struct Arguments {
   int splits;
   bool causal, heads_first;
 };
+
+__device__ __forceinline__ float finite_or_nan(float x) { return __builtin_fmaf(x, 0.0f, x); }
 
 // Bytes at[i] + g of the four strings w[i], for i = 0 .. 3 and every g.
 template <int G, int STEP, int WORDS>
@@ -356,8 +362,11 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
       const bool held = !PACKED || g == my_group;
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int j = 0; j < 8; ++j) {
         v[j] = held ? to_f32(x[32 * g + j]) : 0.0f;
+        if (TQ == 1) // (an infinity's second term is NaN by itself)
+          v[j] = finite_or_nan(v[j]);
+      }
       float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
     }
   }
   const float scale =
-      (p.scale ? p.scale[0] : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
+      (p.scale ? finite_or_nan(p.scale[0]) : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
 
   v4f o[RT][2 * G];
   float top[RT], sum[RT], low[RT][SG]; // low: sum of p m
@@ -824,7 +833,7 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
 
   // This lane's rows: q in the order of a word's codes as they come out of it.
   const float scale =
-      (p.scale ? p.scale[0] : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
+      (p.scale ? finite_or_nan(p.scale[0]) : 1.0f / __builtin_sqrtf((float)D)) * kLog2E;
   v8h q[2][G];
   float by[2]; // a score's factor
   int row_lo[2], row_hi[2];
@@ -854,13 +863,14 @@ __global__ __launch_bounds__(256, G <= 4 ? 2 : 1) void k_cache_prompt(const Argu
     const int up = 14 + 127 - (int)(__builtin_bit_cast(unsigned, most) >> 23);
     // (not 0: what is not seen has the score -inf)
     by[r] = __builtin_fmaxf(__builtin_ldexpf(__builtin_fabsf(scale), -up), 0x1p-126f);
+    const float sign = most == inf ? __builtin_nanf("") : scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int f = 0; f < G; ++f) {
       constexpr int order[4] = {0, 2, 1, 3};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = to_f32(pairs[f][order[e % 4]].v[e / 4]);
-        q[r][f][e] = (_Float16)__builtin_ldexpf(scale < 0.0f ? -v : v, up);
+        q[r][f][e] = (_Float16)__builtin_ldexpf(v * sign, up);
       }
     }
   }

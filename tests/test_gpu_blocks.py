@@ -902,3 +902,30 @@ def test_append_many_rows(om):
     om.CacheAppend4(c, d, d, on(om, np.array([16 - S], np.int32)))
     qc, qs = ref.quantize4(om.to_float32(rows))
     assert all(np.array_equal(g.numpy()[0, 0], w) for g, w in zip(c.tensors, (qc, qs, qc, qs)))
+
+
+@pytest.mark.parametrize("dtype,S", [("f32", 1), ("f16", 1), ("bf16", 1), ("f32", 30), ("f16", 30), ("bf16", 30), ("bf16", 140)])
+def test_attention_of_infinities_that_make_every_score_the_lowest(om, dtype, S):
+    """Scores of -inf alone are a softmax of 0 / 0: NaN, unlike a row that sees no key."""
+    rng = np.random.default_rng(S)
+    c = om.Cache4(3, 1, 200, 128)
+    c.k_codes, c.k_scales = ref.quantize4(rng.uniform(1, 2, (3, 1, 200, 128)).astype(np.float32))
+    c.v_codes, c.v_scales = ref.quantize4(rng.standard_normal((3, 1, 200, 128)).astype(np.float32))
+    c = to_gpu(om, c)
+    past, starts = on(om, np.full(3, 20, np.int32)), on(om, np.array([0, 0, 190], np.int32))
+    x = -rng.uniform(1, 2, (3, 2, S, 128)).astype(np.float32)
+
+    def attend(x, scale=None):
+        return back(om, om.CacheAttention4(on(om, om.from_float32(x, dt(om, dtype))), c, past, starts=starts,
+                                           scale=None if scale is None else on(om, np.float32(scale))))
+
+    plain = attend(x)
+    assert np.isfinite(plain).all() and plain[:2].all() and not plain[2].any()
+    for scale, sign in ((np.inf, 1), (-np.inf, -1)):
+        got = attend(sign * x, scale)
+        assert np.isnan(got[:2]).all() and not got[2].any()
+    bad = np.zeros((3, 2, S), bool)
+    bad[0, 1, 0] = bad[1, 0, S - 1] = True
+    x[bad, 33] = x[2, 0, 0, 5] = -np.inf
+    got = attend(x)
+    assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], plain[~bad])
