@@ -287,7 +287,9 @@ void om_mi355x_RotaryEmbedding(OMTensor *y, const OMTensor *x,
  * sequence b has page b.  past: i32 [B], tokens in front of the new ones.
  * counts: i32 [B], how many of the S rows of a sequence are new tokens, or
  * NULL: all S.  New token i of sequence b is token past[b] + i.
- * Tables, past and counts that lie in host memory are checked (EINVAL); in GPU
+ * Tables, past and counts that lie in host memory are checked (EINVAL), tables as
+ * far as the call reaches: pages in front of the new tokens of an append, or of what
+ * attention's window and starts leave, may be none.  In GPU
  * memory a token without a place in the cache is not stored, and not seen.  No two
  * new tokens may have the same place.  In GPU memory, the cache, q, k, v and y start
  * at a multiple of 16 bytes.  A cache has fewer than 2^32 rows.

@@ -2381,9 +2381,11 @@ struct CacheViews {
     return true;
   }
 
-  // What says where the tokens of B sequences, S new ones of each, lie.
+  // What says where the tokens of B sequences, S new ones of each, lie.  first_of(b,
+  // past): the first of sequence b's that the call reaches.
+  template <typename First>
   bool places(const OMTensor *table_t, const OMTensor *past_t,
-      const OMTensor *counts_t, int64_t B, int64_t S, const char *op) {
+      const OMTensor *counts_t, int64_t B, int64_t S, const char *op, First first_of) {
     has_table = table_t != nullptr;
     has_counts = counts_t != nullptr;
     if (!past_t) {
@@ -2416,15 +2418,17 @@ struct CacheViews {
       fail(EINVAL, "%s: a sequence's pages hold more than 2^30 tokens", op);
       return false;
     }
-    return host_places_ok(B, S, op);
+    return host_places_ok(B, S, op, first_of);
   }
   int64_t capacity() const { return has_table ? table_pages * page_size : page_size; }
 
-  // Host memory can be looked at: every token must have a place.
+  // Host memory can be looked at: every token that the call reaches must have a place
+  // (pages in front of a window may be given back).
   static bool readable(const View &v) {
     return v.data && v.numel > 0 && !backed_lookup(v.data) && !is_device_ptr(v.data);
   }
-  bool host_places_ok(int64_t B, int64_t S, const char *op) const {
+  template <typename First>
+  bool host_places_ok(int64_t B, int64_t S, const char *op, First first_of) const {
     const bool see_past = readable(past), see_counts = has_counts && readable(counts);
     const bool see_table = has_table && readable(table);
     for (int64_t b = 0; b < B; ++b) {
@@ -2442,9 +2446,9 @@ struct CacheViews {
                      "tokens", op, (long long)b, (long long)t, (long long)capacity());
         return false;
       }
-      if (!see_table || (has_counts && !see_counts))
+      if (!see_table || (has_counts && !see_counts) || n == 0)
         continue;
-      for (int64_t j = 0; j * page_size < t + n; ++j) {
+      for (int64_t j = first_of(b, t) / page_size; j * page_size < t + n; ++j) {
         const int64_t page = ((const int32_t *)table.data)[b * table_pages + j];
         if (page < 0 || page >= pages) {
           fail(EINVAL, "%s: page_table[%lld, %lld] is %lld, of %lld pages", op,
@@ -2703,7 +2707,8 @@ void om_mi355x_CacheAppend4(OMTensor *k_codes, OMTensor *k_scales,
   }
   Heads h;
   if (!heads_of(k, cache.H, cache.D, op, "k", h) ||
-      !cache.places(page_table, past, counts, h.B, h.S, op))
+      !cache.places(page_table, past, counts, h.B, h.S, op,
+          [](int64_t, int64_t t) { return t; }))
     return;
   if (k.numel / 64 > kMostBlocks) {
     fail(EINVAL, "%s: k is too large", op);
@@ -2750,8 +2755,15 @@ void om_mi355x_CacheAttention4(OMTensor *y_t, const OMTensor *q_t,
   }
   Heads h;
   if (!heads_of(q, 0, cache.D, op, "q", h) ||
-      !cache.places(page_table, past, counts, h.B, h.S, op) ||
       !per_sequence(starts_t, h.B, op, "starts", starts))
+    return;
+  // (starts that only the GPU knows: the new tokens at least have places)
+  const bool see_starts = starts_t && CacheViews::readable(starts);
+  auto first_key = [&](int64_t b, int64_t t) {
+    const int64_t start = see_starts ? ((const int32_t *)starts.data)[b] : starts_t ? t : 0;
+    return std::max<int64_t>({0, start, window > 0 ? t - window + 1 : 0});
+  };
+  if (!cache.places(page_table, past, counts, h.B, h.S, op, first_key))
     return;
   if (scale_t) {
     if (!view_of(scale_t, "scale", scale))

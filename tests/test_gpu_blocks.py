@@ -929,3 +929,41 @@ def test_attention_of_infinities_that_make_every_score_the_lowest(om, dtype, S):
     x[bad, 33] = x[2, 0, 0, 5] = -np.inf
     got = attend(x)
     assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], plain[~bad])
+
+
+@pytest.mark.parametrize("options", [{"window": 20}, {"starts": [64, 40]}, {"starts": [0, 70], "window": 10}, {"counts": [0, 5], "window": 33}])
+def test_host_tables_of_pages_that_nothing_reaches(om, options):
+    """Pages in front of a window, or of a sequence's start, may be given back: their
+    entries are not looked at, in host memory as on the GPU."""
+    rng = np.random.default_rng(7)
+    B, H, S, D, size, past = 2, 2, 5, 64, 16, np.array([90, 77], np.int32)
+    c = random_cache(om, rng, 13, H, size, D)
+    table = rng.permutation(12).reshape(B, 6).astype(np.int32)
+    k, v, q = (rng.standard_normal((B, h, S, D)).astype(np.float32) for h in (H, H, 2 * H))
+    arrays = {n: np.array(options[n], np.int32) for n in ("counts", "starts") if n in options}
+    window = options.get("window", 0)
+
+    def run(table, put, c):
+        given = {n: put(a) for n, a in arrays.items()}
+        starts = given.pop("starts", None)
+        om.CacheAppend4(c, put(k), put(v), put(past), put(table), **given)
+        return back(om, om.CacheAttention4(put(q), c, put(past), put(table), starts=starts, window=window, out=put(np.zeros_like(q)), **given))
+
+    d = to_gpu(om, c)
+    want = run(table, lambda a: on(om, a), d)
+    short = table.copy()
+    for b in range(B):
+        first = max(0 if "starts" not in options else options["starts"][b], int(past[b]) - window + 1 if window else 0)
+        short[b, :first // size] = [-1, 99][b]
+        if options.get("counts", [S, S])[b] == 0:
+            short[b] = -1
+    assert (short != table).any()
+    assert np.array_equal(run(short, lambda a: a.copy(), c), want)
+    assert all(np.array_equal(h, g.numpy()) for h, g in zip(c.tensors, d.tensors))
+    # starts that only the GPU knows; a page that is needed
+    if "starts" in arrays:
+        got = om.CacheAttention4(q, c, past, short, starts=on(om, arrays["starts"]), window=window)
+        assert np.array_equal(got, want)
+    short[1, past[1] // size] = 13
+    with pytest.raises(om.RuntimeError_, match="page_table\\[1, 4\\] is 13, of 13 pages"):
+        run(short, lambda a: a.copy(), c)
