@@ -967,3 +967,43 @@ def test_host_tables_of_pages_that_nothing_reaches(om, options):
     short[1, past[1] // size] = 13
     with pytest.raises(om.RuntimeError_, match="page_table\\[1, 4\\] is 13, of 13 pages"):
         run(short, lambda a: a.copy(), c)
+
+
+# Keys a wave looks up the places of at once: 4096 in one part.
+@pytest.mark.parametrize("dtype,B,Hq,H,S,D", [
+    ("bf16", 64, 8, 8, 1, 64), ("f32", 64, 32, 8, 1, 64), ("f16", 64, 8, 8, 1, 128),  # columns packed by groups
+    ("f16", 64, 8, 8, 17, 64), ("f32", 64, 8, 8, 1, 96),                               # rows a column
+    ("bf16", 64, 8, 8, 128, 64), ("bf16", 64, 8, 8, 128, 128)])                        # prompts
+def test_attention_of_more_keys_than_places_known_at_once(om, dtype, B, Hq, H, S, D):
+    """Heads enough that their keys are one part, 9000 of them in pages in any order,
+    one beyond the first 4096 missing."""
+    rng = np.random.default_rng(D + S)
+    size, keys, pool = 48, 9000, 300
+    each = -(-(keys + S) // size)
+    c = random_cache(om, rng, pool, H, size, D)
+    table = rng.integers(0, pool, (B, each)).astype(np.int32)
+    missing = 5000 // size + np.arange(B) % 3
+    table[np.arange(B), missing] = -1
+    past = (keys - 37 * (np.arange(B) % 7)).astype(np.int32)
+    q = om.from_float32(rng.standard_normal((B, Hq, S, D)), dt(om, dtype))
+    got = back(om, om.CacheAttention4(on(om, q), to_gpu(om, c), on(om, past), on(om, table)))
+    x = om.to_float32(q).astype(np.float64)
+    K, V = ref.values4(c.k_codes, c.k_scales), ref.values4(c.v_codes, c.v_scales)
+    half = dtype == "bf16" and S >= 128
+    if half:
+        K, V = (t.astype(np.float16).astype(np.float64) for t in (K, V))
+    vsc = np.abs(c.v_scales.astype(np.float64))
+    for b, j, i in [(0, 0, 0), (1, Hq - 1, S - 1), (5, Hq // 2, S // 2), (B - 1, Hq - 1, S - 1), (B - 1, 0, 0)]:
+        t = np.arange(past[b] + i + 1)
+        t = t[t // size != missing[b]]
+        page, slot, g = table[b, t // size], t % size, j * H // Hq
+        k, v = K[page, g, slot], V[page, g, slot]
+        s = k @ x[b, j, i] / np.sqrt(D)
+        p = np.exp(s - s.max())
+        sure = np.array([[[[np.abs(k * x[b, j, i]).sum(-1).max() / np.sqrt(D), np.abs(v).max(),
+                            (vsc[page, g, slot, :, 0] * 15 + vsc[page, g, slot, :, 1]).max(), len(t)]]]])
+        one, want = got[b, j, i][None, None, None], (p @ v / p.sum())[None, None, None]
+        if half:
+            check_prompt(one, want, sure, dtype)
+        else:
+            check_attention(om, one, want, sure, dtype)
