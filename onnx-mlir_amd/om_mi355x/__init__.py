@@ -589,6 +589,8 @@ CACHE_GROUP = 32     # elements under one scale and lowest value (the 4-bit cach
 def from_float32(x, dtype) -> np.ndarray:
     """Host array of ``x`` in ``dtype`` (float32, float16 or bfloat16), rounded to
     nearest even."""
+    if np.dtype(dtype) not in (np.float32, np.float16, bfloat16):
+        raise ValueError(f"from_float32: float32, float16 or bfloat16, not {np.dtype(dtype)}")
     x = np.ascontiguousarray(x, np.float32)
     if np.dtype(dtype) != bfloat16:
         return x.astype(dtype)

@@ -178,3 +178,10 @@ def test_rotary_tables(om):
     for bad in (dict(dim=7), dict(dim=8, factor=0.5), dict(dim=8, scaling="yarn"), dict(dim=8, scaling="other")):
         with pytest.raises(ValueError):
             om.rotary_tables(4, **{"factor": 2.0, **bad})
+
+
+def test_from_float32_refuses_types_that_it_does_not_round_to(om):
+    for dtype in (om.float8_e4m3fn, np.uint8, np.int32, np.float64):
+        with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+            om.from_float32(np.float32([1.5, 300.0]), dtype)
+    assert om.from_float32(np.float32([1.5]), "float16").dtype == np.float16
