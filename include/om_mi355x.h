@@ -267,12 +267,12 @@ void om_mi355x_MatMulBlocks(OMTensor *y, const OMTensor *a,
     const OMTensor *a_scale, const OMTensor *b, const OMTensor *b_scale,
     const OMTensor *bias, int64_t activation);
 
-/* onnx.RotaryEmbedding.  x: float [B, H, S, D], or [B, S, H * D] with num_heads
- * = H; y like x (it may be x).  The first rotary_embedding_dim elements of a
+/* onnx.RotaryEmbedding, with tables in f32 whatever x's type (the ONNX operator's
+ * have x's: such have to be converted, or made by their angles, which loses less).
+ * x: float [B, H, S, D], or [B, S, H * D] with num_heads = H; y like x (it may be x).  The first rotary_embedding_dim elements of a
  * head (0: all) are rotated in pairs, (2 i, 2 i + 1) if interleaved, otherwise
  * (i, i + rotary_embedding_dim / 2), the others pass through.
- * cos_cache, sin_cache: f32 (whatever x's type) [positions,
- * rotary_embedding_dim / 2] with position_ids i64 [B, S], or
+ * cos_cache, sin_cache: f32 [positions, rotary_embedding_dim / 2] with position_ids i64 [B, S], or
  * [B, S, rotary_embedding_dim / 2] with position_ids NULL.  A token whose
  * position the tables do not hold gets NaN. */
 void om_mi355x_RotaryEmbedding(OMTensor *y, const OMTensor *x,

@@ -26,8 +26,9 @@ __device__ __forceinline__ float block_scale(float top) {
 }
 
 // x / s, correctly rounded, in four instructions instead of the divide's
-// eleven where r = RN(1 / s): q0 = RN(x r), e = x - q0 s (exact), q = RN(q0 +
-// e r).  Nothing under- or overflows for scales from 2^-80 to 2^96 and
+// eleven where r = RN(1 / s) (Markstein's correction of a quotient, "Computation of
+// elementary functions on the IBM RISC System/6000", 1990): q0 = RN(x r), e = x - q0 s
+// (exact), q = RN(q0 + e r).  Nothing under- or overflows for scales from 2^-80 to 2^96 and
 // quotients of 2^-11 .. 1024; smaller ones become 0 either way, larger ones do
 // not occur or are infinite, and clamped they give 448, as they would divided.
 // Other scales, an infinite block's among them, take the divide.
@@ -343,8 +344,8 @@ __device__ __forceinline__ void copy16(
 // asked for.  Scales come by way of LDS, once a block: asked for by every wave,
 // the few lines that hold them are what L2 is busiest with.  Products by bf16
 // instructions; sums of the waves meet in LDS in a fixed order.
-// One row, 4096 x 11008: 11.5 us (12.4 with scales asked for by every wave, 11.9
-// with the weights copied into LDS, 9.8 with neither rows of a nor scales).
+// One row, 4096 x 11008: 11.1 us (12.4 with scales asked for by every wave, 11.9
+// with the weights copied into LDS, 9.8 with neither rows of a nor scales); 16 rows 14.7.
 // TAIL: any K and any alignment, what lies past a row's end 0; and any number of
 // rows, 16 MT a blockIdx.y, for products that have no room for aligned copies.
 template <typename T, int MT, int WAVES, int DEPTH, bool TAIL, bool STAGED>
@@ -826,7 +827,7 @@ __global__ __launch_bounds__(256) void k_align_rows(const AlignRows p) {
 // Rows that the kernel for few of them takes: 16, and 32 of small products, where a
 // tile's steps cost more than fetching a's rows in every block (32 rows, skinny /
 // tiles: 768x768 4.5 / 5.5, 2048x2048 7.5 / 7.5, 4096x1024 9.2 / 8.3, 4096x11008
-// 26 / 14 us).
+// 26 / 13.5 us).
 bool few_rows(int64_t M, int64_t K, int64_t N) {
   return M <= 16 || (M <= 32 && K * N < (int64_t)1 << 21);
 }
@@ -864,9 +865,11 @@ constexpr int kUnaligned = kTileForms; // no tiles: rows that they cannot copy
 //   base + steps (full rounds * full + the rest of the fullest CU * lone) + rounds * round
 //   [+ 3.7 + 1.43 us per million sums of all parts, to write, read and add them]
 // microseconds, where a CU holds per_cu tiles at once and takes its share of them
-// one round after the other.  Fitted to 872 products of 80 .. 4096 rows timed in
-// every form (relative errors 6 - 10 %); the forms that it takes are 1.4 % slower
-// than the fastest in the geometric mean, 14 % at most.
+// one round after the other.  Fitted to 84 products of 80 .. 4096 rows timed in every
+// form (872 times), when a CU held two tiles of 64 x 128; it holds three now.  Of the
+// same products on the kernels as they are, its times are off by 8 - 11 % (root mean
+// square), and the forms that it takes are 2.1 % slower than the fastest in the
+// geometric mean, 17 % at most (128 rows, where 64 x 128 in more parts is faster).
 struct TileCost {
   int bm, bn, per_cu;
   float base, full, lone, round;

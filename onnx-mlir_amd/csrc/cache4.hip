@@ -725,8 +725,8 @@ __global__ __launch_bounds__(kWaves * 64, PACKED && G * RT <= 4 ? 2 : 1) void k_
 // keys 4 h .. of either 16, element 16 t + c in the order z (4 G) + j: byte z / 2 of
 // word j, z % 2 its half.  All are read as they lie, 1024 bytes after one another.
 //
-// 2048 rows on 4096 keys, 32 heads on 8 of 128, causal: 142 us, 730 TFLOP/s (534 us in
-// tiles).  Bound by instructions: vector ones take 48 % of the clocks (of some 300 for 64
+// 2048 rows on 4096 keys, 32 heads on 8 of 128, causal: 140 us, 735 TFLOP/s (534 us in
+// tiles); heads of 256, 16 on 4, 251 us: they spill 21 registers.  Bound by instructions: vector ones take 48 % of the clocks (of some 300 for 64
 // keys a wave, 130 make its share of them and 32 are exponentials at a quarter of the
 // rate), matrix ones 28 %, and the two blocks that a CU has registers for overlap little;
 // blocks of unequal length leave it with one for the rest.
