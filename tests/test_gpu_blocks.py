@@ -1081,3 +1081,36 @@ def test_matmul_blocks_mean_error_of_8_bit_sums(om, outliers, most):
     off = np.abs(back(om, got) - want.astype(np.float16).astype(np.float64)).mean() / np.sqrt((want ** 2).mean())
     print("mean error of the sums: %.2e" % off)
     assert off <= most
+
+
+@pytest.mark.parametrize("dtype,S", [("f32", 3), ("bf16", 3), ("bf16", 150)])
+def test_a_cache_whose_offsets_pass_32_bits(om, dtype, S):
+    """2^26 rows of 128 bytes: the last pages give what a small cache gives."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(S)
+    pages, size, D, each = 2 ** 19, 64, 256, 5
+    big = to_gpu(om, om.Cache4(1, 1, 16, D))
+    memory = {}
+    for name, per, kind in (("codes", D // 2, np.uint8), ("scales", D // 8, np.float16)):
+        for x in "kv":
+            t = memory[x + name] = torch.zeros((pages * 2 * size, per), dtype=torch.uint8, device="cuda")
+            shape = (pages, 2, size, D // 2) if kind == np.uint8 else (pages, 2, size, D // 32, 2)
+            setattr(big, x + "_" + name, om.DeviceArray.wrap(t.data_ptr(), shape, np.dtype(kind), owner=t))
+    torch.cuda.synchronize()
+    small = to_gpu(om, om.Cache4(each, 2, size, D))
+    for x in ("k_codes", "k_scales", "v_codes", "v_scales"):
+        t = getattr(small, x)
+        setattr(small, x, on(om, np.zeros((each, 2, size) + ((D // 2,) if "codes" in x else (D // 32, 2)), t.dtype)))
+    order = rng.permutation(each).astype(np.int32)
+    k, v = (om.from_float32(rng.standard_normal((1, 2, 300, D)), dt(om, dtype)) for _ in range(2))
+    q = on(om, om.from_float32(rng.standard_normal((1, 2, S, D)), dt(om, dtype)))
+    past = on(om, np.array([300 - S], np.int32))
+    got = []
+    for c, first in ((big, pages - each), (small, 0)):
+        table = on(om, order[None] + np.int32(first))
+        om.CacheAppend4(c, on(om, k), on(om, v), on(om, np.zeros(1, np.int32)), table)
+        got.append(back(om, om.CacheAttention4(q, c, past, table)))
+    # (parts are as many as the pages of a sequence allow: the same)
+    assert got[0].any() and np.array_equal(got[0], got[1])
+    om.synchronize()
+    assert not any(t[: (pages - each) * 2 * size].any() for t in memory.values())
