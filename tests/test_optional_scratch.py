@@ -107,7 +107,10 @@ class _BlockGemm(ctypes.Structure):
                [(n, ctypes.c_int) for n in ("kind", "activation")] + [(n, ctypes.c_void_p) for n in ("rows", "parts")]
 
 
-@pytest.mark.parametrize("M,K,N,wants", BLOCK_PRODUCTS + [(33, 129, 1001, "any K"), (1000, 16, 40, "neither")])
+@pytest.mark.parametrize("M,K,N,wants", BLOCK_PRODUCTS + [
+    (33, 129, 1001, "any K"), (1000, 16, 40, "neither"),
+    (70, 33001, 40, "both"),          # more scales than LDS has room for
+    (2 ** 21 + 37, 17, 1, "any K")])  # more rows than one launch takes
 def test_block_products_without_room_for_scratch(rt, M, K, N, wants):
     """The launch as the runtime makes it where there is no memory for the copies, the
     sums, or either."""
