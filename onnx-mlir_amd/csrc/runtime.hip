@@ -2289,6 +2289,11 @@ constexpr int64_t kMostBlocks = ((int64_t)1 << 31) - 1;
 
 int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
+// Scales hold a row's blocks beside one another: flat, or in rows of them.
+bool in_rows_of(const View &scale, int64_t blocks) {
+  return scale.numel == 0 || scale.rank < 2 || scale.shape[scale.rank - 1] == blocks;
+}
+
 // Heads as [B, H, S, D], or [B, S, H * D] (`heads` or `dim` given).
 struct Heads {
   int64_t B = 0, S = 0, H = 0, D = 0;
@@ -2524,6 +2529,10 @@ void om_mi355x_DynamicQuantizeBlocks(OMTensor *y_t, OMTensor *scale_t,
         (long long)sc.numel, (long long)scales);
     return;
   }
+  if (!in_rows_of(sc, blocks_of(K))) {
+    fail(EINVAL, "%s: y_scale must be [.., %lld]", op, (long long)blocks_of(K));
+    return;
+  }
   if (K > kMostOfOne || scales > kMostBlocks) {
     fail(EINVAL, "%s: x is too large", op);
     return;
@@ -2576,7 +2585,8 @@ void om_mi355x_MatMulBlocks(OMTensor *y_t, const OMTensor *a_t,
   }
   if (as.dtype != OM_MI355X_TYPE_FLOAT || bs.dtype != OM_MI355X_TYPE_FLOAT ||
       as.numel != g.M * blocks_of(g.K) ||
-      bs.numel != blocks_of(g.N) * blocks_of(g.K)) {
+      bs.numel != blocks_of(g.N) * blocks_of(g.K) ||
+      !in_rows_of(as, blocks_of(g.K)) || !in_rows_of(bs, blocks_of(g.K))) {
     fail(EINVAL, "%s: scales must be f32, a_scale [.., %lld] and b_scale "
                  "[%lld, %lld]", op, (long long)blocks_of(g.K),
         (long long)blocks_of(g.N), (long long)blocks_of(g.K));

@@ -185,3 +185,12 @@ def test_from_float32_refuses_types_that_it_does_not_round_to(om):
         with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
             om.from_float32(np.float32([1.5, 300.0]), dtype)
     assert om.from_float32(np.float32([1.5]), "float16").dtype == np.float16
+
+
+def test_scales_the_other_way_round_are_refused(om):
+    """As many entries, but not blocks of a row beside one another."""
+    a, b = f8(om, 4, 200), f8(om, 300, 200)
+    refused(om, "a_scale \\[.., 2\\]", lambda: om.MatMulBlocks(a, f32(2, 4), b, f32(3, 2)))
+    refused(om, "b_scale \\[3, 2\\]", lambda: om.MatMulBlocks(a, f32(4, 2), b, f32(2, 3)))
+    refused(om, "y_scale must be \\[.., 2\\]", lambda: om.DynamicQuantizeBlocks(f32(4, 200), out=(a, f32(2, 4))))
+    refused(om, "y_scale must be \\[.., 2\\]", lambda: om.DynamicQuantizeBlocks(f32(300, 200), 128, out=(b, f32(2, 3))))
