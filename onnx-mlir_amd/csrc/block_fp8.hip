@@ -1040,10 +1040,9 @@ hipError_t launch_block_gemm(hipStream_t s, const BlockGemm &g) {
   p.parts = 1;
   p.part_blocks = p.kblocks;
   TilePlan plan = {};
-  if (few_rows(g.M, g.K, g.N)) {
-  } else if (!g.rows && block_gemm_row_bytes(g)) {
+  if (!g.rows && block_gemm_row_bytes(g)) {
     plan.form = kUnaligned;
-  } else {
+  } else if (!few_rows(g.M, g.K, g.N)) {
     plan = plan_tiles(g, g.parts ? kMostParts : 1);
     p.parts = plan.parts;
     p.part_blocks = (p.kblocks + plan.parts - 1) / plan.parts;
